@@ -62,6 +62,15 @@ def draw(rng):
 
 
 # --------------------------------------------------------------------------------------------------------- 8 bits
+def _two32(k):
+    """2^k in 32 bits for whole k in [-126, 127], from its bits (a library's power need not be exact)."""
+    return ((k.int() + 127) << 23).view(torch.float32)
+
+
+def _two64(k):
+    return ((k.long() + 1023) << 52).view(torch.float64)
+
+
 def _q8(x):
     """8-bit values (in 32 bits, to be multiplied by their scales) and the scales' exponents, of [rows, columns] fp32."""
     rows, cols = x.shape
@@ -71,13 +80,13 @@ def _q8(x):
     m, e = torch.frexp(amax)  # amax = m 2^e, m in [0.5, 1): the least k with amax <= 448 2^k = 0.875 2^(k + 9)
     k = torch.clamp(e - 9 + (m > 0.875).int(), min=-126)
     k = torch.where(amax > 0, k, torch.full_like(k, -126))
-    v = torch.ldexp(g, -k.unsqueeze(-1)).to(torch.float8_e4m3fn)
+    v = (g * _two32(-k.unsqueeze(-1))).to(torch.float8_e4m3fn)
     return v.view(rows, -1)[:, :cols].contiguous(), (k + 127).to(torch.uint8)
 
 
 def _dq8(v, b):
     rows, cols = v.shape
-    s = torch.ldexp(torch.ones((), device=v.device), b.int() - 127).repeat_interleave(GROUP, 1)[:, :cols]
+    s = _two32(b.int() - 127).repeat_interleave(GROUP, 1)[:, :cols]
     return v.float() * s
 
 
@@ -295,7 +304,7 @@ def _grid8(v):
     """v (64 bits) at the nearest values of 4 exponent and 3 fraction bits, ties to even: steps of 2^-3 of the leading
     power of two, 2^-9 below 2^-6."""
     _, e = torch.frexp(v)
-    step = torch.pow(2.0, torch.clamp(e.double() - 1, min=-6.0) - 3.0)
+    step = _two64(torch.clamp(e - 1, min=-6) - 3)
     return torch.round(v / step) * step
 
 
@@ -305,7 +314,7 @@ def _exact_q8(y):
         part = y[:, at:at + GROUP]
         top = part.abs().amax(1, keepdim=True)
         k = torch.ceil(torch.log2(torch.clamp(top, min=1e-300) / 448.0))
-        scale = torch.pow(2.0, torch.clamp(k, min=-126.0))
+        scale = _two64(torch.clamp(k, min=-126.0))
         parts.append(_grid8(part / scale) * scale)
     return torch.cat(parts, 1)
 
@@ -314,7 +323,7 @@ def _exact_read(pair):
     v, b = pair
     v, b = v.reshape(-1, v.shape[-1]), b.reshape(-1, b.shape[-1])
     col = torch.arange(v.shape[1], device=v.device) // GROUP
-    return v.double() * torch.pow(2.0, b.double() - 127.0)[:, col]
+    return v.double() * _two64(b.long() - 127)[:, col]
 
 
 def exact(case, seed):
