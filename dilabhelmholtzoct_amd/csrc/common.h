@@ -55,10 +55,10 @@ __device__ __forceinline__ float erf_fast(float x) {
   const float y = 1.0f - p * t * __expf(-ax * ax);
   return copysignf(y, x);
 }
-// GELU on the same A&S erf, rearranged so that a pair of values runs on packed f32 arithmetic: with
+// GELU on the same A&S erf, rearranged so that a pair of values runs side by side: with
 // z = |x|/sqrt2, t = 1/(1 + p z), q = P(t) t exp(-x^2/2) (so erf(z) = 1 - q), GELU(x) = max(x, 0) - |x q / 2|
 // (x >= 0: x - x q/2; x < 0: x q/2). The 1/2 is folded into P's coefficients (exact). gelu_fast and
-// gelu_fast2 run the same operation sequence (packed FMA/MUL round like their scalar forms), so every GEMM
+// gelu_fast2 run the same operation sequence (FMA/MUL per element), so every GEMM
 // epilogue — scalar or pairwise — gives bit-identical outputs.
 namespace gelu_c {
 constexpr float P = 0.3275911f * 0.70710678118654752f, A1 = 0.5f * 0.254829592f, A2 = 0.5f * -0.284496736f,

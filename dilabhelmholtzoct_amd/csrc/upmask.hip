@@ -118,7 +118,7 @@ __device__ __forceinline__ int pix_local(int rr, int s) {
   const int x1l = rr >> 2, dy1 = (rr >> 1) & 1, dx1 = rr & 1;
   return (2 * dy1 + (s >> 1)) * 128 + 4 * x1l + 2 * dx1 + (s & 1);
 }
-// GELU (erf form) and its derivative on two values at once (packed f32: v_pk_fma / v_pk_mul / v_pk_add, the
+// GELU (erf form) and its derivative on two values at once (the
 // kernels are VALU-bound), one shared erf / exp evaluation (A&S 7.1.26, |err| <= 1.5e-7)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return __builtin_elementwise_fma(a, b, c); }

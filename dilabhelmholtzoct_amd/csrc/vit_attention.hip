@@ -432,7 +432,7 @@ __global__ __launch_bounds__(THR) void vit_attn_global_kernel(const E* __restric
     // once per tile: p = exp2(c1 * acc + (rh - m)), one FMA + one exp per score
     const float rh = relh[tile * 32 + l32];
     // max: 16 three-input maxima (scores are finite: the kernel is built without NaN canonicalisation, see
-    // Makefile); sum: packed adds
+    // Makefile); sum: pairwise adds
     float mx = sacc[0][0];
 #pragma unroll
     for (int i = 1; i < 31; i += 2) mx = max3f(mx, sacc[i >> 4][i & 15], sacc[(i + 1) >> 4][(i + 1) & 15]);
@@ -446,11 +446,11 @@ __global__ __launch_bounds__(THR) void vit_attn_global_kernel(const E* __restric
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         const f32x2 x = {sacc[t2][r], sacc[t2][r + 1]};
-        const f32x2 y = x * c1 + c;  // v_pk_fma_f32
+        const f32x2 y = x * c1 + c;
         const f32x2 pv = {__builtin_amdgcn_exp2f(y[0]), __builtin_amdgcn_exp2f(y[1])};
         sacc[t2][r] = pv[0];
         sacc[t2][r + 1] = pv[1];
-        ls2 += pv;  // v_pk_add_f32
+        ls2 += pv;
       }
     l_run += ls2[0] + ls2[1];
 #pragma unroll
@@ -574,11 +574,11 @@ __global__ __launch_bounds__(THR4, HALF ? 3 : 2) void vit_attn_global4_kernel(co
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         const f32x2 x = {sacc[t2][r], sacc[t2][r + 1]};
-        const f32x2 y = x * c1 + c;  // v_pk_fma_f32
+        const f32x2 y = x * c1 + c;
         const f32x2 pv = {__builtin_amdgcn_exp2f(y[0]), __builtin_amdgcn_exp2f(y[1])};
         sacc[t2][r] = pv[0];
         sacc[t2][r + 1] = pv[1];
-        ls2 += pv;  // v_pk_add_f32
+        ls2 += pv;
       }
     l_run += ls2[0] + ls2[1];
 #pragma unroll
@@ -610,11 +610,11 @@ __device__ __forceinline__ void softmax_pack(f32x16 (&s)[2], float c1, float c, 
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
       const f32x2 x = {s[t2][r], s[t2][r + 1]};
-      const f32x2 y = x * c1 + c;  // v_pk_fma_f32
+      const f32x2 y = x * c1 + c;
       const f32x2 pv = {__builtin_amdgcn_exp2f(y[0]), __builtin_amdgcn_exp2f(y[1])};
       s[t2][r] = pv[0];
       s[t2][r + 1] = pv[1];
-      ls2 += pv;  // v_pk_add_f32
+      ls2 += pv;
     }
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) pf[ks] = pack8<E>(s[ks >> 1], 8 * (ks & 1));
@@ -895,11 +895,11 @@ __global__ __launch_bounds__(WTHR, HD == 64 ? 3 : 2) void vit_attn_window_kernel
       for (int r = 0; r < 16; r += 2) {
         const float cc = r < 8 ? c0 : cc1;
         const f32x2 x = {sacc[t2][r], sacc[t2][r + 1]};
-        const f32x2 y = x * c1 + (f32x2){cc, cc};  // v_pk_fma_f32
+        const f32x2 y = x * c1 + (f32x2){cc, cc};
         const f32x2 pv = {__builtin_amdgcn_exp2f(y[0]), __builtin_amdgcn_exp2f(y[1])};
         sacc[t2][r] = pv[0];
         sacc[t2][r + 1] = pv[1];
-        ls2 += pv;  // v_pk_add_f32
+        ls2 += pv;
       }
     }
     l_run += ls2[0] + ls2[1];
