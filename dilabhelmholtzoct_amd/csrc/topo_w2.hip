@@ -351,6 +351,8 @@ __global__ void __launch_bounds__(256) w2_loss_kernel(const int32_t* __restrict_
 
 }  // namespace
 
+static __global__ void clear_status_kernel(int32_t* status) { *status = 0; }
+
 extern "C" int64_t octsam_topo_w2_workspace(int32_t Kn, int32_t max_pairs) {
   if (Kn <= 0 || max_pairs <= 0) return 0;
   const W2Layout L(max_pairs);
@@ -389,7 +391,7 @@ extern "C" int octsam_topo_w2(const int32_t* pairs, const int32_t* cnt, const fl
   int32_t* match = (int32_t*)(ws + (size_t)Kn * 8);
   int32_t* status = (int32_t*)(ws + (size_t)Kn * 8 + (size_t)Kn * max_pairs * 4);
   char* gscratch = ws + ((((size_t)Kn * 8 + (size_t)Kn * max_pairs * 4 + 16) + 255) & ~(size_t)255);
-  (void)hipMemsetAsync(status, 0, 4, s);
+  hipLaunchKernelGGL(clear_status_kernel, dim3(1), dim3(1), 0, s, status);  // (a kernel: graphs replay it in order)
   if (lds) {
     static int attr_set = 0;
     if (!attr_set) {
