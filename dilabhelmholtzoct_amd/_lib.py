@@ -15,7 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # OCTSAM_LIB: another build of the same ABI (A/B diagnostics in scripts/, never set by the package itself)
 LIB_PATH = os.environ.get("OCTSAM_LIB") or os.path.join(_HERE, "liboctsam_hip.so")
 
-ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 
 c_void_p = ctypes.c_void_p
 c_int32 = ctypes.c_int32
@@ -66,6 +66,25 @@ _SIGNATURES = {
     "octsam_layernorm_bwd": (c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_int32, c_int64, c_int32, c_void_p, c_int32, c_float,
                                        c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
+    "octsam_quant8": (c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int64,
+                                c_void_p]),
+    "octsam_dequant8": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int64,
+                                  c_void_p]),
+    "octsam_rmsnorm_fwd": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int32,
+                                     c_float, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64,
+                                     c_void_p, c_int64, c_void_p, c_void_p]),
+    "octsam_rmsnorm_bwd_workspace": (c_int64, [c_int64, c_int32]),
+    "octsam_rmsnorm_bwd": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64,
+                                     c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int32,
+                                     c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "octsam_gated_fwd": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32, c_int32,
+                                   c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64,
+                                   c_void_p]),
+    "octsam_gated_bwd_workspace": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    "octsam_gated_bwd": (c_int32, [c_void_p, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_int32,
+                                   c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32,
+                                   c_int32, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_void_p,
+                                   c_void_p, c_int64, c_void_p]),
     "octsam_relu_bwd": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
     "octsam_group_sum": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_int64, c_void_p, c_void_p]),
     "octsam_vit_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,

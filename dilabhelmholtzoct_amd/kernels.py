@@ -234,6 +234,263 @@ def layernorm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: t
     return dx, dw, db
 
 
+# ---- 8-bit checkpoints, RMS norm, gated unit: tensors are [..., columns] with contiguous columns and, in two dimensions,
+# any row stride of at least their width; every launch goes to the operands' device, on its current stream
+
+_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+_Q8 = 3  # the 8-bit form's type code
+
+
+def _type(t, what):
+    ty = _TYPES.get(t.dtype)
+    if ty is None:
+        raise ValueError(f"{what} is {t.dtype}: bf16, fp32 or fp16 is expected")
+    return ty
+
+
+def _rows(t, what):
+    """(rows, columns, row stride) of t seen as rows of its last dimension."""
+    shape = t.shape
+    if len(shape) == 2:
+        rows, cols = shape
+        ld, sc = t.stride()
+        if sc != 1 and cols > 1:
+            raise ValueError(f"{what}: columns must be contiguous")
+        if rows <= 1:
+            ld = cols
+        elif ld < cols:
+            raise ValueError(f"{what}: rows overlap (row stride {ld}, width {cols})")
+        return rows, cols, ld
+    if not shape or not t.is_contiguous():
+        raise ValueError(f"{what}: [rows, columns] with any row stride, or contiguous [..., columns]")
+    cols = shape[-1]
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    return rows, cols, cols
+
+
+def _like(t, rows, cols, what):
+    """Row stride of t, which must be [rows, cols]."""
+    r, c, ld = _rows(t, what)
+    if r != rows or c != cols:
+        raise ValueError(f"{what} is {tuple(t.shape)}: {rows} rows of {cols} are expected")
+    return ld
+
+
+def _vector(t, n, what):
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous fp32 with {n} elements")
+
+
+def _q8_pair(pair, rows, cols, what):
+    """(q, row stride, scale, scale row stride) of an 8-bit pair that must be [rows, cols]."""
+    q, scale = pair
+    if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8:
+        raise ValueError(f"{what}: an 8-bit pair is (float8_e4m3fn values, uint8 scales), got {q.dtype}, {scale.dtype}")
+    return q, _like(q, rows, cols, what), scale, _like(scale, rows, (cols + 31) // 32, what + " scales")
+
+
+def _device_of(*ts):
+    """The one device that all given tensors are on."""
+    dev = None
+    for t in ts:
+        if t is not None:
+            if not t.is_cuda:
+                raise ValueError("octsam kernels take device tensors only")
+            if dev is None:
+                dev = t.device
+            elif t.device != dev:
+                raise ValueError(f"octsam kernels take tensors of one device, got {dev} and {t.device}")
+    return dev
+
+
+def _call_on(dev, name, *args):
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args)
+
+
+def q8_empty(shape, device) -> tuple[torch.Tensor, torch.Tensor]:
+    """An unfilled 8-bit pair for [..., columns] values: float8_e4m3fn values of that shape and uint8 scales
+    [..., ceil(columns / 32)] (scale byte b stands for 2^(b - 127) and multiplies 32 consecutive columns)."""
+    shape = tuple(shape)
+    return (torch.empty(shape, device=device, dtype=torch.float8_e4m3fn),
+            torch.empty(shape[:-1] + ((shape[-1] + 31) // 32,), device=device, dtype=torch.uint8))
+
+
+def quant8(x: torch.Tensor, q8=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The 8-bit form of x ([..., columns], bf16 / fp32 / fp16): (values, scales), written into q8 when given; see
+    octsam_quant8. Non-finite elements become NaN and do not touch their group's other values."""
+    if q8 is None:
+        q8 = q8_empty(x.shape, x.device)
+    dev = _device_of(x, *q8)
+    rows, cols, ldx = _rows(x, "x")
+    q, ldq, scale, lds = _q8_pair(q8, rows, cols, "q8")
+    _call_on(dev, "octsam_quant8", ptr(x), _type(x, "x"), ldx, rows, cols, ptr(q), ldq, ptr(scale), lds)
+    return q8
+
+
+def dequant8(q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """out = the values an 8-bit pair stands for (exact in fp32 and bf16 down to 2^-126; fp16 rounds once)."""
+    dev = _device_of(q, scale, out)
+    rows, cols, ldo = _rows(out, "out")
+    q, ldq, scale, lds = _q8_pair((q, scale), rows, cols, "q")
+    _call_on(dev, "octsam_dequant8", ptr(q), ldq, ptr(scale), lds, rows, cols, ptr(out), _type(out, "out"), ldo)
+    return out
+
+
+def rmsnorm_fwd(x: torch.Tensor, w: torch.Tensor, eps: float, out: torch.Tensor | None = None, *,
+                residual: torch.Tensor | None = None, sum_out: torch.Tensor | None = None, q8=None,
+                rstd: torch.Tensor | None = None) -> torch.Tensor | None:
+    """out = RMS norm of s = x + residual over the last dim, times w (fp32); see octsam_rmsnorm_fwd. residual: x's type or
+    fp32; sum_out receives s in residual's type (it may be x or residual itself, in place); q8: an 8-bit pair that
+    receives out's values; rstd: fp32 [rows], for the backward. Every output is optional."""
+    q, scale = q8 if q8 is not None else (None, None)
+    dev = _device_of(x, w, out, residual, sum_out, q, scale, rstd)
+    rows, D, ldx = _rows(x, "x")
+    xt = _type(x, "x")
+    _vector(w, D, "w")
+    ldr = lds = ldy = ldq = ldsc = 0
+    rt = yt = 0
+    if residual is not None:
+        ldr, rt = _like(residual, rows, D, "residual"), _type(residual, "residual")
+    if sum_out is not None:
+        if residual is None or sum_out.dtype != residual.dtype:
+            raise ValueError("rmsnorm_fwd: sum_out needs a residual and has its type")
+        lds = _like(sum_out, rows, D, "sum_out")
+    if out is not None:
+        ldy, yt = _like(out, rows, D, "out"), _type(out, "out")
+    if q8 is not None:
+        q, ldq, scale, ldsc = _q8_pair(q8, rows, D, "q8")
+    if rstd is not None:
+        _vector(rstd, rows, "rstd")
+    _call_on(dev, "octsam_rmsnorm_fwd", ptr(x), xt, ldx, ptr(residual), rt, ldr, ptr(w), rows, D, float(eps), ptr(sum_out),
+             lds, ptr(out), yt, ldy, ptr(q), ldq, ptr(scale), ldsc, ptr(rstd))
+    return out
+
+
+def rmsnorm_bwd(dy: torch.Tensor, s, rstd: torch.Tensor, w: torch.Tensor, dx: torch.Tensor, *,
+                dres: torch.Tensor | None = None, dw: torch.Tensor | None = None):
+    """Gradients of rmsnorm_fwd: returns (dx, dw). s: the sum that was normalised (x without a residual), or an 8-bit pair
+    of it; rstd from the forward; dx (the gradient of x and of residual) = the norm's gradient + dres (dx's type: what
+    arrives at the sum from the residual stream); it may be dy or dres itself, in place. dw fp32, overwritten."""
+    s8 = isinstance(s, (tuple, list))
+    sv, sc = s if s8 else (s, None)
+    dev = _device_of(dy, sv, sc, rstd, w, dx, dres, dw)
+    rows, D, lddy = _rows(dy, "dy")
+    if s8:
+        sv, lds, sc, ldsc = _q8_pair(s, rows, D, "s")
+        st = _Q8
+    else:
+        lds, ldsc, st = _like(sv, rows, D, "s"), 0, _type(sv, "s")
+    _vector(rstd, rows, "rstd")
+    _vector(w, D, "w")
+    lddx, xt = _like(dx, rows, D, "dx"), _type(dx, "dx")
+    lddres = 0
+    if dres is not None:
+        if dres.dtype != dx.dtype:
+            raise ValueError("rmsnorm_bwd: dres has dx's type")
+        lddres = _like(dres, rows, D, "dres")
+    if dw is None:
+        dw = torch.empty(D, device=dev, dtype=torch.float32)
+    else:
+        _vector(dw, D, "dw")
+    nbytes = _lib.load().octsam_rmsnorm_bwd_workspace(rows, D)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    _call_on(dev, "octsam_rmsnorm_bwd", ptr(dy), _type(dy, "dy"), lddy, ptr(sv), st, lds, ptr(sc), ldsc, ptr(rstd), ptr(w),
+             rows, D, ptr(dres), lddres, ptr(dx), xt, lddx, ptr(dw), ptr(ws), nbytes)
+    return dx, dw
+
+
+def _e16(t, what):
+    if t.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what} is {t.dtype}: bf16 or fp16 is expected")
+    return _TYPES[t.dtype]
+
+
+def _kept(kept, ty, rows, F, what):
+    """(tensor, type, row stride, scale, scale row stride) of the kept projections: [rows, 2F] of type ty, or an 8-bit
+    pair [rows, 2, F]."""
+    if isinstance(kept, (tuple, list)):
+        q, scale = kept
+        if q.dim() != 3 or scale.dim() != 3 or q.shape[0] != rows:
+            raise ValueError(f"{what}: an 8-bit pair [{rows}, 2, {F}] is expected")
+        _q8_pair(kept, 2 * rows, F, what)
+        return q, _Q8, 2 * F, scale, 2 * ((F + 31) // 32)
+    if _TYPES.get(kept.dtype) != ty:
+        raise ValueError(f"{what} is {kept.dtype}: the operands' type or an 8-bit pair is expected")
+    return kept, ty, _like(kept, rows, 2 * F, what), None, 0
+
+
+def gated_fwd(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, act: int = _lib.ACT_SILU,
+              bias: torch.Tensor | None = None, save=None) -> torch.Tensor:
+    """out = act(g) * u with [g | u] = x w^T + bias: x [M, D], w [2F, D] (gate rows first), out [M, F], all bf16 or all fp16;
+    bias fp32 [2F]; D and F multiples of 8. save keeps g and u for gated_bwd: [M, 2F] of x's type, or an 8-bit pair
+    q8_empty((M, 2, F)); see octsam_gated_fwd."""
+    sv, sc = save if isinstance(save, (tuple, list)) else (save, None)
+    dev = _device_of(x, w, out, bias, sv, sc)
+    ty = _e16(x, "x")
+    if w.dtype != x.dtype or out.dtype != x.dtype:
+        raise ValueError("gated_fwd: x, w and out have one type")
+    M, D, ldx = _rows(x, "x")
+    n2, _, ldw = _rows(w, "w")
+    F = n2 // 2
+    if w.dim() != 2 or n2 % 2 or w.shape[1] != D:
+        raise ValueError(f"w is {tuple(w.shape)}: [2F, {D}] is expected")
+    ldh = _like(out, M, F, "out")
+    if bias is not None:
+        _vector(bias, 2 * F, "bias")
+    st = ldsv = ldsc = 0
+    if save is not None:
+        sv, st, ldsv, sc, ldsc = _kept(save, ty, M, F, "save")
+    _call_on(dev, "octsam_gated_fwd", ptr(x), ldx, ptr(w), ldw, ptr(bias), M, D, F, act, ty, ptr(out), ldh, ptr(sv), st, ldsv,
+             ptr(sc), ldsc)
+    return out
+
+
+def gated_bwd(dh: torch.Tensor, saved, x, w: torch.Tensor, *, act: int = _lib.ACT_SILU, dx: torch.Tensor | None = None,
+              dw: torch.Tensor | None = None, db: torch.Tensor | None = None, h: torch.Tensor | None = None) -> None:
+    """Gradients of gated_fwd, written into the outputs that are given: dx [M, D], dw [2F, D] (x's 16-bit type or fp32),
+    db fp32 [2F], and h = act(g) * u again. saved: gated_fwd's save; x: its input, or an 8-bit pair of it (only dw reads
+    it: None without dw); see octsam_gated_bwd."""
+    sv, sc = saved if isinstance(saved, (tuple, list)) else (saved, None)
+    xv, xs = x if isinstance(x, (tuple, list)) else (x, None)
+    dev = _device_of(dh, sv, sc, xv, xs, w, dx, dw, db, h)
+    ty = _e16(dh, "dh")
+    M, F, lddh = _rows(dh, "dh")
+    n2, D, ldw = _rows(w, "w")
+    if w.dim() != 2 or n2 != 2 * F or w.dtype != dh.dtype:
+        raise ValueError(f"w is {w.dtype} {tuple(w.shape)}: {dh.dtype} [{2 * F}, D] is expected")
+    sv, st, ldsv, sc, ldsc = _kept(saved, ty, M, F, "saved")
+    xt = ldx = ldxs = lddx = lddw = ldh = wt = 0
+    if dw is not None:
+        if x is None:
+            raise ValueError("gated_bwd: dw needs x")
+        if xs is not None:
+            xv, ldx, xs, ldxs = _q8_pair(x, M, D, "x")
+            xt = _Q8
+        else:
+            ldx, xt = _like(xv, M, D, "x"), ty
+            if xv.dtype != dh.dtype:
+                raise ValueError("gated_bwd: x has dh's type or is an 8-bit pair")
+        lddw, wt = _like(dw, 2 * F, D, "dw"), _type(dw, "dw")
+    if dx is not None:
+        lddx = _like(dx, M, D, "dx")
+    if h is not None:
+        ldh = _like(h, M, F, "h")
+    if (dx is not None and dx.dtype != dh.dtype) or (h is not None and h.dtype != dh.dtype):
+        raise ValueError("gated_bwd: dx and h have dh's type")
+    if db is not None:
+        _vector(db, 2 * F, "db")
+    nbytes = _lib.load().octsam_gated_bwd_workspace(M, D, F, int(xt == _Q8))
+    ws = torch.empty(max(nbytes, 16), device=dev, dtype=torch.uint8)
+    _call_on(dev, "octsam_gated_bwd", ptr(dh), lddh, ptr(sv), st, ldsv, ptr(sc), ldsc, ptr(xv), xt, ldx, ptr(xs), ldxs, ptr(w),
+             ldw, M, D, F, act, ty, ptr(h), ldh, ptr(dx), lddx, ptr(dw), wt, lddw, ptr(db), ptr(ws), nbytes)
+
+
 def vit_attention(qkv: torch.Tensor, out: torch.Tensor, rel_pos_h: torch.Tensor, rel_pos_w: torch.Tensor, *,
                   nseq: int, side: int, heads: int, grid: int = 0,
                   pad_row: torch.Tensor | None = None) -> torch.Tensor:

@@ -31,6 +31,7 @@ extern "C" {
 #define OCTSAM_ACT_NONE 0
 #define OCTSAM_ACT_RELU 1
 #define OCTSAM_ACT_GELU 2
+#define OCTSAM_ACT_SILU 3 /* x * sigmoid(x): the gated unit only */
 
 /* ---------------------------------------------------------------- library */
 int octsam_abi_version(void);
@@ -171,6 +172,57 @@ int octsam_layernorm_bwd(const void* dy, int32_t dy_f32, const void* x, int32_t 
                          const float* rstd, const float* w, const float* b, int32_t act, int64_t rows, int32_t D,
                          void* dx, int32_t dx_f32, float beta, void* dx2_bf16, float* dw_part, float* db_part,
                          int32_t nblocks, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit activation checkpoints
+ * The library's 8-bit form of a row of C values: C e4m3 bytes and ceil(C / 32) scale bytes; byte b multiplies its 32
+ * consecutive columns by 2^(b - 127) (the last group of a row may be shorter). Written: b = the smallest (>= 1) with
+ * the group's largest finite |x| <= 448 * 2^(b - 127); values rounded to nearest even; a non-finite x becomes NaN.
+ * Element types of these and the following entries (*_type): 0 bf16, 1 fp32, 2 fp16, 3 the 8-bit form (where named).
+ * ld*: elements (bytes for 8-bit operands and scales) between rows, at least the row's width. Rows of a width that is
+ * a multiple of 8 at 16-B (8-bit: 8-B) aligned addresses and strides of a multiple of 8 take the vector kernels; any
+ * other layout of elements at their natural alignment is served element by element. rows = 0 does nothing. */
+int octsam_quant8(const void* x, int32_t x_type, int64_t ldx, int64_t rows, int32_t cols, void* q, int64_t ldq,
+                  void* scale, int64_t ld_scale, void* stream);
+int octsam_dequant8(const void* q, int64_t ldq, const void* scale, int64_t ld_scale, int64_t rows, int32_t cols, void* y,
+                    int32_t y_type, int64_t ldy, void* stream);
+
+/* ---------------------------------------------------------------- RMS norm with the residual's addition
+ * Forward: s = x + r (r optional: x's type or fp32); rstd = (mean(s^2) + eps)^(-1/2); y = s * rstd * w from the
+ * unrounded fp32 s. Outputs, each optional: sum_out (s in r's type; needs r), y (any type), q / scale (y in the 8-bit
+ * form), rstd (fp32 [rows]). sum_out may be x or r and y may be x, in place (same address, type and stride).
+ * Backward from the stored s (any type, or 8-bit with s_scale): dx = dres + rstd * (g - n * mean(g * n)), g = dy * w,
+ * n = s * rstd, the gradient of x and of r; dres (optional, dx's type) is what arrives at s from the residual stream,
+ * and dx may be dy or dres in place; dw[c] = sum over rows of dy * n (fp32, overwritten; fixed order of additions).
+ * workspace: octsam_rmsnorm_bwd_workspace(rows, D) bytes, 16-B aligned. */
+int octsam_rmsnorm_fwd(const void* x, int32_t x_type, int64_t ldx, const void* r, int32_t r_type, int64_t ldr,
+                       const float* w, int64_t rows, int32_t D, float eps, void* sum_out, int64_t ld_sum, void* y,
+                       int32_t y_type, int64_t ldy, void* q, int64_t ldq, void* scale, int64_t ld_scale, float* rstd,
+                       void* stream);
+int64_t octsam_rmsnorm_bwd_workspace(int64_t rows, int32_t D);
+int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy, const void* s, int32_t s_type, int64_t lds,
+                       const void* s_scale, int64_t ld_scale, const float* rstd, const float* w, int64_t rows, int32_t D,
+                       const void* dres, int64_t lddres, void* dx, int32_t dx_type, int64_t lddx, float* dw,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- gated feed-forward unit
+ * Forward: [g | u] = x W^T + bias, h = act(g) * u. x [M, D], W [2F, D] (F gate rows, then F up rows), h [M, F], all of
+ * `type` (0 bf16, 2 fp16); bias fp32 [2F] or NULL; act OCTSAM_ACT_*. save (optional) keeps g and u for the backward:
+ * [M, 2F] of `type`, or (save_type 3) 8-bit [M, 2, F] with scales [M, 2, ceil(F / 32)]; ld_save, ld_scale are the
+ * strides of M. D and F are multiples of 8; rows start at multiples of 16 bytes (8 for 8-bit operands).
+ * Backward from the kept g, u (gu_type = type or 3): dg = dh * u * act'(g), du = dh * act(g); outputs, each optional:
+ * h = act(g) * u again (for the weight gradient of the layer behind), dx = [dg | du] W (of `type`),
+ * dw = [dg | du]^T x (fp32 or `type`; x of `type` or 8-bit, x_type 3), db = column sums of [dg | du] (fp32 [2F]).
+ * Outputs are overwritten and must not overlap inputs. Fixed order of additions: the same bits every run. M = 0 gives
+ * zero dw and db. workspace: octsam_gated_bwd_workspace(M, D, F, x_type == 3) bytes, 16-B aligned. */
+int octsam_gated_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, int64_t M, int32_t D,
+                     int32_t F, int32_t act, int32_t type, void* h, int64_t ldh, void* save, int32_t save_type,
+                     int64_t ld_save, void* save_scale, int64_t ld_scale, void* stream);
+int64_t octsam_gated_bwd_workspace(int64_t M, int32_t D, int32_t F, int32_t x_q8);
+int octsam_gated_bwd(const void* dh, int64_t lddh, const void* gu, int32_t gu_type, int64_t ldgu, const void* gu_scale,
+                     int64_t ld_gu_scale, const void* x, int32_t x_type, int64_t ldx, const void* x_scale,
+                     int64_t ld_x_scale, const void* w, int64_t ldw, int64_t M, int32_t D, int32_t F, int32_t act,
+                     int32_t type, void* h, int64_t ldh, void* dx, int64_t lddx, void* dw, int32_t dw_type, int64_t lddw,
+                     float* db, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- ViT attention
  * Replaces SamVisionAttention.forward + get_decomposed_rel_pos (hf:modeling_sam.py:729-882).

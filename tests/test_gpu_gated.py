@@ -1,0 +1,504 @@
+"""RMS norm with the residual's addition, the gated feed-forward unit and the 8-bit checkpoints against plain 64-bit
+statements (tests/gated_ref.py). Tolerances: half a step of the output's type per rounding, plus fp32 error terms that
+scale with the sums of magnitudes of what is added."""
+import pytest
+import torch
+
+import gated_ref as ref
+from gated_ref import U32, half_step, tiny
+
+pytestmark = pytest.mark.gpu
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def k(cuda):
+    from dilabhelmholtzoct_amd import kernels
+    return kernels
+
+
+def rnd(seed, *shape, scale=1.0, dtype=F32):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def padded(rows, cols, dtype, pad=8, off=0, fill=7.0):
+    """A [rows, cols] view with row stride cols + pad that starts `off` elements into a buffer of `fill`, and the buffer."""
+    buf = torch.full(((rows + 2) * (cols + pad) + off,), fill, device="cuda").to(dtype)
+    return buf[off + cols + pad:].as_strided((rows, cols), (cols + pad, 1)), buf
+
+
+def untouched(view, buf, fill=7.0):
+    """Whether everything of buf outside view still holds `fill`."""
+    mask = torch.ones(buf.numel(), dtype=torch.bool, device="cuda")
+    rows, cols = view.shape
+    mask.as_strided((rows, cols), view.stride(), view.storage_offset()).zero_()
+    return bool((buf.float()[mask] == fill).all())
+
+
+def close(got, want, tol):
+    got, want = got.double(), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    bad = (got - want).abs() > tol
+    bad &= ~torch.isnan(want)
+    assert not bool(bad.any()), (int(bad.sum()), float(((got - want).abs() / tol.clamp(min=1e-300))[bad].max()))
+
+
+# ------------------------------------------------------------------------------------------------------------- 8 bits
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 8), (3, 31), (2, 32), (5, 33), (7, 40), (129, 256), (64, 251), (2, 4096)])
+def test_q8_bits(k, dtype, rows, cols):
+    x = rnd(rows * 1000 + cols, rows, cols, dtype=dtype)
+    q, s = k.quant8(x)
+    v, want = ref.q8(x)
+    assert torch.equal(s, want)
+    assert torch.equal(q.double(), v)  # from exact inputs the rounding is a definition
+    for out_t in (F32, BF):
+        out = k.dequant8(q, s, torch.empty(rows, cols, device="cuda", dtype=out_t))
+        assert torch.equal(out.double(), ref.q8_value(v, want))  # exact: 4 significant bits
+    err = (ref.q8_value(v, want) - x.double()).abs()
+    top = torch.nn.functional.pad(x.double().abs(), (0, -cols % 32)).view(rows, -1, 32).amax(-1).repeat_interleave(32, 1)[:, :cols]
+    assert bool((err <= 2.0 ** -4 * x.double().abs() + top * 2.0 ** -17).all())  # half a step; below, e4m3's subnormals
+
+
+def test_q8_borders(k):
+    """Ties to even, the largest value, the border between two scales, subnormals, zeros, infinities and NaN."""
+    row = torch.zeros(12, 32, device="cuda")
+    row[0, :8] = torch.tensor([448.0, 440.0, 424.0, 17.0, 19.0, 1.0625, 1.1875, -1.0625])  # ties of e4m3 at scale 1
+    row[1, 0] = 448.0000305  # the next fp32 value above: the scale doubles
+    row[2, 0] = 3.4e38
+    row[3, 0] = 1e-44  # an fp32 subnormal: scale at its floor
+    row[4, :3] = torch.tensor([float("inf"), 1.0, -2.0])
+    row[5, :3] = torch.tensor([float("nan"), -float("inf"), 3.0])
+    row[6, :] = float("nan")
+    row[7, :4] = torch.tensor([448.0, 2.0 ** -9, 2.0 ** -10, 1.5 * 2.0 ** -9])  # the smallest step and its ties
+    row[8, 31] = -5.0
+    row[9, :2] = torch.tensor([-0.0, 0.0])
+    row[10, :] = 1.75
+    row[11, :] = 1.7500001
+    q, s = k.quant8(row)
+    v, want = ref.q8(row)
+    assert torch.equal(s, want)
+    assert torch.equal(torch.nan_to_num(q.double(), nan=-7e9), torch.nan_to_num(v, nan=-7e9))
+    assert torch.equal(torch.isnan(k.dequant8(q, s, torch.empty_like(row))), torch.isnan(v))
+
+
+def test_dequant8_every_byte_and_scale(k):
+    q = torch.arange(256, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn).repeat(256, 1)
+    s = torch.arange(256, dtype=torch.uint8, device="cuda")[:, None].repeat(1, 8).contiguous()
+    want = ref.q8_value(q, s)
+    got = k.dequant8(q, s, torch.empty(256, 256, device="cuda"))
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    fin = ~torch.isnan(want)
+    assert torch.equal(got[fin], want[fin].float())
+
+
+def test_q8_strides_and_guard(k):
+    for cols, off in ((64, 0), (64, 3), (40, 1), (33, 0)):
+        xv, _ = padded(9, cols, BF, off=off)
+        xv.copy_(rnd(cols, 9, cols, dtype=BF))
+        qb = torch.full((11 * (cols + 8),), 0x38, dtype=torch.uint8, device="cuda")
+        q = qb[cols + 8:].view(torch.float8_e4m3fn).as_strided((9, cols), (cols + 8, 1))
+        sb = torch.full((11, 7), 9, dtype=torch.uint8, device="cuda")
+        s = sb[1:10, :(cols + 31) // 32]
+        k.quant8(xv, (q, s))
+        v, want = ref.q8(xv)
+        assert torch.equal(q.double(), v) and torch.equal(s, want)
+        assert bool((sb[:, (cols + 31) // 32:] == 9).all()) and bool((sb[[0, 10]] == 9).all())
+        m = torch.ones_like(qb, dtype=torch.bool)
+        m.as_strided((9, cols), (cols + 8, 1), cols + 8).zero_()
+        assert bool((qb[m] == 0x38).all())
+        out, buf = padded(9, cols, F32, off=off)
+        k.dequant8(q, s, out)
+        assert torch.equal(out.double(), ref.q8_value(v, want)) and untouched(out, buf)
+
+
+# --------------------------------------------------------------------------------------------------------------- norm
+NORM_SHAPES = [(1, 1), (1, 8), (3, 64), (5, 128), (2, 136), (17, 251), (33, 256), (1029, 251), (4, 520), (300, 1024), (65, 1280),
+               (2, 2048), (3, 2056), (2, 8192), (2, 8200), (1, 20000)]
+
+
+@pytest.mark.parametrize("rows,d", NORM_SHAPES)
+@pytest.mark.parametrize("xt,rt,yt", [(BF, None, BF), (BF, BF, BF), (BF, F32, BF), (F16, F16, F32), (F32, F32, F16), (F16, F32, F16),
+                                      (F32, None, BF)])
+def test_norm_fwd(k, rows, d, xt, rt, yt):
+    eps = 1e-6
+    x = rnd(rows + d, rows, d, scale=2.0, dtype=xt)
+    r = rnd(rows + d + 1, rows, d, dtype=rt) if rt else None
+    w = 1 + 0.2 * rnd(3, d)
+    y, rstd = torch.empty(rows, d, device="cuda", dtype=yt), torch.empty(rows, device="cuda")
+    s = torch.empty(rows, d, device="cuda", dtype=rt) if rt else None
+    q8 = k.q8_empty((rows, d), "cuda")
+    assert k.rmsnorm_fwd(x, w, eps, y, residual=r, sum_out=s, q8=q8, rstd=rstd) is y
+    ws, wr, wy = ref.norm_fwd(x, w, eps, r)
+    # the squares' sum: at most 128 additions in a chain (the vector kernels hold 32 values a lane, the others up to
+    # d / 64) and the joining shuffles; the root halves it; then one rounding each for the two products and the root
+    c = (d / 64 + 64) * U32
+    close(rstd, wr, wr * c)
+    close(y, wy, wy.abs() * (half_step(yt) + c) + tiny(yt))
+    if rt:
+        close(s, ws, ws.abs() * (half_step(rt) + U32) + tiny(rt))
+    # the 8-bit form: half a step of e4m3 against the exact y, plus y's own error; below the normals, half of 2^-9 of the
+    # scale, which is at most the group's largest / 224
+    top = torch.nn.functional.pad(wy.abs(), (0, -d % 32)).view(rows, -1, 32).amax(-1).repeat_interleave(32, 1)[:, :d]
+    close(ref.q8_value(*q8), wy, wy.abs() * (2.0 ** -4 + 2 * c) + top * (1 + c) * 2.0 ** -10 / 224)
+    # an output that is not asked for changes nothing of the others
+    y2 = torch.empty_like(y)
+    k.rmsnorm_fwd(x, w, eps, y2, residual=r)
+    assert torch.equal(y, y2)
+    only = k.q8_empty((rows, d), "cuda")
+    k.rmsnorm_fwd(x, w, eps, residual=r, q8=only)
+    assert torch.equal(only[0].view(torch.uint8), q8[0].view(torch.uint8)) and torch.equal(only[1], q8[1])
+
+
+@pytest.mark.parametrize("d,off", [(256, 0), (256, 1), (250, 0)])
+def test_norm_fwd_views_and_in_place(k, d, off):
+    rows = 37
+    x, xb = padded(rows, d, BF, off=off)
+    x.copy_(rnd(1, rows, d, dtype=BF))
+    r = rnd(2, rows, d, dtype=BF)
+    w = 1 + 0.1 * rnd(3, d)
+    y, yb = padded(rows, d, BF, off=off)
+    s, sb = padded(rows, d, BF, off=off)
+    k.rmsnorm_fwd(x, w, 1e-6, y, residual=r, sum_out=s)
+    assert untouched(y, yb) and untouched(s, sb) and untouched(x, xb)
+    want_s, want_y = s.clone(), y.clone()
+    r2 = r.clone()
+    y2 = torch.empty(rows, d, device="cuda", dtype=BF)
+    k.rmsnorm_fwd(x, w, 1e-6, y2, residual=r2, sum_out=r2)  # the stream updated in place
+    assert torch.equal(r2, want_s) and torch.equal(y2, want_y)
+    x2 = x.contiguous()
+    k.rmsnorm_fwd(x2, w, 1e-6, x2, residual=r)
+    assert torch.equal(x2, want_y)
+
+
+def test_norm_fwd_special_values(k):
+    d = 96
+    x = rnd(5, 6, d)
+    x[1] = 0.0
+    x[2, 3] = float("nan")
+    x[3, 4] = float("inf")
+    x[4] *= 1e-30
+    x[5] *= 1e18
+    w = torch.ones(d, device="cuda")
+    y = torch.empty_like(x)
+    k.rmsnorm_fwd(x, w, 1e-6, y)
+    _, _, want = ref.norm_fwd(x, w, 1e-6)
+    assert bool((y[1] == 0).all()) and bool(y[2].isnan().all())
+    assert bool(y[3, 4].isnan()) and bool((y[3, :4] == 0).all())  # inf * 0, and finite * 0
+    close(y[[0, 4]], want[[0, 4]], want[[0, 4]].abs() * 1e-5)
+    close(y[5], want[5], want[5].abs() * 1e-5)
+
+
+@pytest.mark.parametrize("rows,d", NORM_SHAPES + [(0, 256), (5000, 64)])
+@pytest.mark.parametrize("dt,st,xt,res", [(BF, BF, BF, True), (BF, "q8", BF, False), (F32, "q8", F32, True), (F16, F32, F16, True),
+                                          (BF, F32, F32, True), (F32, F16, BF, False)])
+def test_norm_bwd(k, rows, d, dt, st, xt, res):
+    w = 1 + 0.2 * rnd(3, d)
+    s = rnd(rows + d, rows, d, scale=2.0)
+    rstd = torch.rsqrt(s.square().mean(-1) + 1e-6)
+    if st == "q8":
+        kept = k.quant8(s)
+        s = ref.q8_value(*kept)
+    else:
+        kept = s = s.to(st)
+    dy = rnd(rows + d + 2, rows, d, dtype=dt)
+    dres = rnd(rows + d + 3, rows, d, dtype=xt) if res else None
+    dx = torch.empty(rows, d, device="cuda", dtype=xt)
+    got, dw = k.rmsnorm_bwd(dy, kept, rstd, w, dx, dres=dres)
+    assert got is dx
+    wx, ww, size, wsize = ref.norm_bwd(dy, s, rstd, w, dres)
+    close(dx, wx, wx.abs() * half_step(xt) + size * (d / 64 + 64) * U32 + tiny(xt))
+    close(dw, ww, wsize * (rows + 64) * U32)
+    dx2 = dy.clone() if dt == xt else torch.empty_like(dx)
+    dw2 = torch.full((d,), float("nan"), device="cuda")
+    k.rmsnorm_bwd(dx2 if dt == xt else dy, kept, rstd, w, dx2, dres=dres, dw=dw2)  # in place over dy; dw overwritten
+    assert torch.equal(dx, dx2) and torch.equal(dw, dw2)
+    if res:
+        k.rmsnorm_bwd(dy, kept, rstd, w, dres, dres=dres)
+        assert torch.equal(dx, dres)
+
+
+def test_norm_bwd_views(k):
+    for d, off in ((256, 0), (256, 1), (100, 0)):
+        rows = 50
+        dy, _ = padded(rows, d, BF, off=off)
+        dy.copy_(rnd(1, rows, d, dtype=BF))
+        s = rnd(2, rows, d, dtype=BF)
+        rstd = torch.rsqrt(s.float().square().mean(-1) + 1e-6)
+        w = 1 + 0.1 * rnd(3, d)
+        dx, xb = padded(rows, d, BF, off=off)
+        _, dw = k.rmsnorm_bwd(dy, s, rstd, w, dx)
+        wx, ww, size, wsize = ref.norm_bwd(dy, s, rstd, w)
+        close(dx, wx, wx.abs() * half_step(BF) + size * 80 * U32 + tiny(BF))
+        close(dw, ww, wsize * (rows + 64) * U32)
+        assert untouched(dx, xb)
+
+
+def test_norm_gradient_against_differences(k):
+    """d(sum of dy * y) along random directions of x and w, central differences of the 64-bit forward."""
+    rows, d = 9, 72
+    x, w, dy = rnd(1, rows, d), 1 + 0.3 * rnd(2, d), rnd(3, rows, d)
+    rstd, y = torch.empty(rows, device="cuda"), torch.empty(rows, d, device="cuda")
+    k.rmsnorm_fwd(x, w, 1e-5, y, rstd=rstd)
+    dx, dw = k.rmsnorm_bwd(dy, x, rstd, w, torch.empty_like(x))
+    f = lambda a, b: float((ref.norm_fwd(a, b, 1e-5)[2] * dy.double()).sum())  # noqa: E731
+    vx, vw, h = rnd(4, rows, d).double(), rnd(5, d).double(), 1e-5
+    num = (f(x.double() + h * vx, w) - f(x.double() - h * vx, w)) / (2 * h)
+    assert abs(num - float((dx.double() * vx).sum())) <= 1e-4 * float((dx.double() * vx).abs().sum())
+    num = (f(x.double(), w.double() + h * vw) - f(x.double(), w.double() - h * vw)) / (2 * h)
+    assert abs(num - float((dw.double() * vw).sum())) <= 1e-4 * float((dw.double() * vw).abs().sum())
+
+
+# -------------------------------------------------------------------------------------------------------------- gated
+def exact_operands(seed, M, D, F, dtype):
+    """Small multiples of powers of two, so that g and u are exact in fp32 (|sums| < 2^24 steps) whatever the order."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    ints = lambda *s: torch.randint(-4, 5, s, generator=g, device="cuda").float()  # noqa: E731
+    x, w = ints(M, D) * 0.25, ints(2 * F, D) * 2.0 ** -5
+    return x.to(dtype), w.to(dtype), ints(2 * F) * 0.125
+
+
+def code(name):
+    from dilabhelmholtzoct_amd import _lib
+    return {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU, "silu": _lib.ACT_SILU}[name]
+
+
+GATED_SHAPES = [(1, 8, 8), (1, 256, 688), (2, 72, 40), (7, 264, 96), (16, 1280, 344), (17, 64, 32), (33, 320, 360), (64, 128, 64),
+                (65, 136, 72), (130, 512, 200), (257, 200, 264), (1029, 256, 688), (300, 768, 1032), (768, 72, 1288),
+                (2100, 328, 520)]
+
+
+@pytest.mark.parametrize("M,D,F", GATED_SHAPES)
+@pytest.mark.parametrize("dtype,act,save,bias", [(BF, "silu", "8", True), (BF, "gelu", "16", False), (F16, "gelu", "8", True),
+                                                 (F16, "silu", "16", True), (BF, "relu", None, True), (F16, "none", None, False)])
+def test_gated_fwd(k, M, D, F, dtype, act, save, bias):
+    x, w, b = exact_operands(M + D + F, M, D, F, dtype)
+    b = b if bias else None
+    out, ob = padded(M, F, dtype)
+    kept = None
+    if save == "8":
+        kept = k.q8_empty((M, 2, F), "cuda")
+    elif save == "16":
+        kept, kb = padded(M, 2 * F, dtype)
+    assert k.gated_fwd(x, w, out, act=code(act), bias=b, save=kept) is out
+    gu, h = ref.gated_fwd(x, w, act, b)
+    g, u = gu[:, :F], gu[:, F:]
+    # g, u exact; the activation to a few fp32 steps (fp16 and bf16 outputs are half a step off at most)
+    close(out, h, h.abs() * half_step(dtype) + (g.abs() + 1) * u.abs() * 8 * U32 + tiny(dtype))
+    assert untouched(out, ob)
+    if save == "16":
+        assert torch.equal(kept.float(), gu.to(dtype).float()) and untouched(kept, kb)
+    elif save == "8":
+        v, s = ref.q8(gu.view(2 * M, F))
+        assert torch.equal(kept[1].view(2 * M, -1), s)
+        assert torch.equal(kept[0].view(2 * M, F).double(), v)
+
+
+@pytest.mark.parametrize("M,D,F", [(1, 1280, 3416), (5, 1024, 2736), (40, 768, 2048), (1029, 256, 688), (1500, 768, 1000)])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_gated_fwd_real_values(k, M, D, F, dtype):
+    x, w, b = rnd(1, M, D, dtype=dtype), rnd(2, 2 * F, D, scale=D ** -0.5, dtype=dtype), 0.1 * rnd(3, 2 * F)
+    out = torch.empty(M, F, device="cuda", dtype=dtype)
+    k.gated_fwd(x, w, out, bias=b)
+    gu, h = ref.gated_fwd(x, w, "silu", b)
+    e = (x.double().abs() @ w.double().abs().t() + b.abs()) * (D + 2) * U32  # fp32 sums of D products, any order
+    g, u = gu[:, :F], gu[:, F:]
+    tol = h.abs() * half_step(dtype) + 1.1 * u.abs() * e[:, :F] + ref.act("silu", g).abs() * e[:, F:] + (g.abs() + 1) * u.abs() * 8 * U32
+    close(out, h, tol + tiny(dtype))
+    assert float((out.double() - h).norm() / h.norm()) <= half_step(dtype)
+
+
+def check_bwd(got, want, dh, gu, x, w, dtype, M, F):
+    """dx and dw: half a step of the output, half a step for each [dg | du] on its way into the product (of the subnormals'
+    step below the normals: gradients are small in fp16) after the activation's error below, fp32 sums; and as norms, where independent roundings do not add up, one step. db: fp32 sums of values whose activation part is off by an
+    absolute 6 fp32 half steps at most besides the relative ones, since terms cancel in it. GELU's slope: the distribution
+    function from erf by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7, halved: 1.3) evaluated with four roundings of
+    values up to 1 (halved: 2), g * density <= 0.25 with an exponential off by 4 (1), their sum's rounding (1); SiLU's
+    p (1 + g (1 - p)): each factor off by three, products up to 0.3 where the sum cancels. It multiplies dh * u in dg, and
+    dh * g in du."""
+    hs = half_step(dtype)
+    a, dh, g, u = want["dgu"].abs(), dh.double().abs(), gu.double()[:, :F], gu.double()[:, F:]
+    if "h" in got:
+        close(got["h"], want["h"], want["h"].abs() * hs + (g.abs() + 1) * u.abs() * 8 * U32 + tiny(dtype))
+    slack = torch.cat([dh * u.abs(), dh * g.abs()], 1) * 6 * U32  # of each [dg | du], before it is rounded
+    off = (a + slack) * hs + slack + tiny(dtype)
+    for name, size, err, n in (("dx", a @ w.double().abs(), off @ w.double().abs(), 2 * F),
+                               ("dw", a.t() @ x.double().abs(), off.t() @ x.double().abs(), M)):
+        if name in got:
+            own = half_step(got[name].dtype)
+            close(got[name], want[name], want[name].abs() * own + err + size * (n + 16) * U32 + tiny(dtype))
+            if want[name].numel() and float(want[name].norm()) > 0:
+                assert float((got[name].double() - want[name]).norm() / want[name].norm()) <= 2 * hs
+    if "db" in got:
+        close(got["db"], want["db"], a.sum(0) * (M + 32) * U32 + slack.sum(0) + 1e-30)
+
+
+@pytest.mark.parametrize("M,D,F", GATED_SHAPES + [(0, 64, 40)])
+@pytest.mark.parametrize("dtype,act,kept,x8,dwt", [(BF, "silu", "8", True, BF), (BF, "gelu", "16", False, F32),
+                                                   (F16, "gelu", "8", True, F16), (F16, "silu", "16", False, F16),
+                                                   (BF, "relu", "16", True, BF), (BF, "none", "8", False, BF)])
+def test_gated_bwd(k, M, D, F, dtype, act, kept, x8, dwt):
+    x, w = rnd(1, M, D, dtype=dtype), rnd(2, 2 * F, D, scale=D ** -0.5, dtype=dtype)
+    dh, gu = rnd(3, M, F, dtype=dtype), rnd(4, M, 2 * F, dtype=dtype)
+    if kept == "8":
+        saved = tuple(t.view(M, 2, t.shape[1]) for t in k.quant8(gu.view(2 * M, F)))
+        gu = ref.q8_value(*saved).view(M, 2 * F)
+    else:
+        saved = gu
+    xin = k.quant8(x) if x8 else x
+    xv = ref.q8_value(*xin) if x8 else x
+    got, bufs = {}, {}
+    for name, rows, cols, t in (("h", M, F, dtype), ("dx", M, D, dtype), ("dw", 2 * F, D, dwt)):
+        got[name], bufs[name] = padded(rows, cols, t)
+    got["db"] = torch.full((2 * F,), float("nan"), device="cuda")
+    k.gated_bwd(dh, saved, xin, w, act=code(act), **got)
+    want = ref.gated_bwd(dh, gu, xv, w, act)
+    check_bwd(got, want, dh, gu, xv, w, dtype, M, F)
+    for name, buf in bufs.items():
+        assert untouched(got[name], buf)
+    # each output alone: the same bits
+    for name in got:
+        one = torch.full_like(got[name].contiguous(), float("nan"))
+        k.gated_bwd(dh, saved, xin if name == "dw" else None, w, act=code(act), **{name: one})
+        assert torch.equal(one, got[name]), name
+
+
+def test_gated_zero_and_special(k):
+    """Zero rows give zeros; NaN and infinity in one row stay in that row (and in dw's and db's sums)."""
+    M, D, F = 70, 64, 48
+    x, w = rnd(1, M, D, dtype=BF), rnd(2, 2 * F, D, scale=0.125, dtype=BF)
+    x[0] = 0.0
+    clean = torch.empty(M, F, device="cuda", dtype=BF)
+    k.gated_fwd(x, w, clean)
+    assert bool((clean[0] == 0).all())
+    x2 = x.clone()
+    x2[5, 3], x2[66, 0] = float("nan"), float("inf")
+    out = torch.empty_like(clean)
+    k.gated_fwd(x2, w, out)
+    rest = [i for i in range(M) if i not in (5, 66)]
+    assert torch.equal(out[rest], clean[rest]) and bool(out[5].isnan().all())
+    assert not bool(torch.isfinite(out[66]).all())
+
+
+def test_gated_gradient_against_differences(k):
+    """d(sum of dh * h) along random directions of x, w and b: central differences of the 64-bit forward against the fp16
+    kernels' gradients; the bound is their rounding (half a step of each of three roundings, on the sum of magnitudes)."""
+    M, D, F = 40, 64, 48
+    x, w, b = rnd(1, M, D, dtype=F16), rnd(2, 2 * F, D, scale=0.125, dtype=F16), 0.1 * rnd(3, 2 * F)
+    dh = rnd(4, M, F, dtype=F16)
+    saved = torch.empty(M, 2 * F, device="cuda", dtype=F16)
+    k.gated_fwd(x, w, torch.empty(M, F, device="cuda", dtype=F16), act=code("gelu"), bias=b, save=saved)
+    dx, dw, db = torch.empty_like(x), torch.empty(2 * F, D, device="cuda"), torch.empty(2 * F, device="cuda")
+    k.gated_bwd(dh, saved, x, w, act=code("gelu"), dx=dx, dw=dw, db=db)
+    f = lambda *a: float((ref.gated_fwd(a[0], a[1], "gelu", a[2])[1] * dh.double()).sum())  # noqa: E731
+    at, e = (x.double(), w.double(), b.double()), 1e-5
+    for i, grad in enumerate((dx, dw, db)):
+        v = rnd(10 + i, *grad.shape).double()
+        up, dn = list(at), list(at)
+        up[i], dn[i] = at[i] + e * v, at[i] - e * v
+        num = (f(*up) - f(*dn)) / (2 * e)
+        assert abs(num - float((grad.double() * v).sum())) <= 8 * half_step(F16) * float((grad.double() * v).abs().sum())
+
+
+# ----------------------------------------------------------------------------------------------------------- together
+def block(k, x, r, wn, w1, b1, w2, dy, eight):
+    """One pre-norm gated block, forward and backward, as a training loop uses it: s = x + r, y = s + W2 gated(norm(s))."""
+    M, D = x.shape
+    F = w1.shape[0] // 2
+    dev, t = x.device, x.dtype
+    n, s, rstd = torch.empty_like(x), torch.empty_like(x), torch.empty(M, device=dev)
+    n8 = k.q8_empty((M, D), dev) if eight else None
+    k.rmsnorm_fwd(x, wn, 1e-6, n, residual=r, sum_out=s, q8=n8, rstd=rstd)
+    kept = k.q8_empty((M, 2, F), dev) if eight else torch.empty(M, 2 * F, device=dev, dtype=t)
+    h = torch.empty(M, F, device=dev, dtype=t)
+    k.gated_fwd(n, w1, h, act=code("silu"), bias=b1, save=kept)
+    y = torch.empty_like(x)
+    k.gemm(h, w2, M=M, N=D, K=F, out=y, residual=s)
+    s8 = k.quant8(s) if eight else s
+    dh = torch.empty_like(h)
+    k.gemm(dy, w2, M=M, N=F, K=D, b_mode=1, out=dh)
+    dn, dw1, db1 = torch.empty_like(x), torch.empty_like(w1), torch.empty(2 * F, device=dev)
+    h2 = torch.empty_like(h)
+    k.gated_bwd(dh, kept, n8 if eight else n, w1, act=code("silu"), dx=dn, dw=dw1, db=db1, h=h2)
+    dw2 = torch.empty(D, F, device=dev)
+    k.gemm(dy, h2, M=D, N=F, K=M, a_mode=1, b_mode=1, out=dw2)
+    dx, dwn = k.rmsnorm_bwd(dn, s8, rstd, wn, torch.empty_like(x), dres=dy)
+    return {"y": y, "dx": dx, "dwn": dwn, "dw1": dw1, "db1": db1, "dw2": dw2}
+
+
+def block_inputs(M=328, D=256, F=688, dtype=BF, seed=0):
+    return (rnd(seed + 1, M, D, dtype=dtype), rnd(seed + 2, M, D, dtype=dtype), 1 + 0.2 * rnd(seed + 3, D),
+            rnd(seed + 4, 2 * F, D, scale=D ** -0.5, dtype=dtype), 0.1 * rnd(seed + 5, 2 * F),
+            rnd(seed + 6, D, F, scale=F ** -0.5, dtype=dtype), rnd(seed + 7, M, D, scale=0.1, dtype=dtype))
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_block_together(k, eight):
+    """The operators in a row against autograd of the same block in 64 bits. Each bf16 rounding on the way adds at most half
+    a step of relative norm (six on the longest path: n, g/u, [dg|du], h, dh, the result); e4m3 keeps 2^-4."""
+    args = block_inputs()
+    got = block(k, *args, eight)
+    x, r, wn, w1, b1, w2 = (a.double().requires_grad_() for a in args[:6])
+    s = x + r
+    n = s * (s.square().mean(-1, keepdim=True) + 1e-6) ** -0.5 * wn
+    gu = n @ w1.t() + b1
+    f = gu.shape[1] // 2
+    y = s + (torch.nn.functional.silu(gu[:, :f]) * gu[:, f:]) @ w2.t()
+    y.backward(args[6].double())
+    want = {"y": y.detach(), "dx": x.grad, "dwn": wn.grad, "dw1": w1.grad, "db1": b1.grad, "dw2": w2.grad}
+    for name, v in want.items():
+        rel = float((got[name].double() - v).norm() / v.norm())
+        tol = 6 * half_step(BF) + (2 * 2.0 ** -4 if eight and name != "y" else 0)
+        assert rel <= tol, (name, rel, tol)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_block_repeats_streams_and_graphs(k, eight):
+    """The same bits again, on another stream, and from a captured graph replayed between eager passes on new inputs."""
+    args = block_inputs(M=1029)
+    first = block(k, *args, eight)
+    again = block(k, *args, eight)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = block(k, *args, eight)
+    torch.cuda.current_stream().wait_stream(side)
+    for name in first:
+        assert torch.equal(first[name], again[name]) and torch.equal(first[name], other[name]), name
+    fixed = [a.clone() for a in args]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block(k, *fixed, eight)
+    for seed in (0, 100, 200):
+        new = block_inputs(M=1029, seed=seed)
+        for a, b in zip(fixed, new):
+            a.copy_(b)
+        graph.replay()
+        want = block(k, *new, eight)
+        torch.cuda.synchronize()
+        for name in want:
+            assert torch.equal(out[name], want[name]), (seed, name)
+
+
+def test_two_graphs_share_nothing(k):
+    """Two captured backward passes, replayed alternately on two streams, keep their own workspaces."""
+    sets = []
+    for seed in (1, 50):
+        args = block_inputs(M=200, seed=seed)
+        want = block(k, *args, True)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = block(k, *args, True)
+        sets.append((g, out, want, torch.cuda.Stream(), args))  # (the graph reads args: they stay alive)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, _, _, st, _ in sets:
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, out, want, _, _ in sets:
+        for name in want:
+            assert torch.equal(out[name], want[name]), name
