@@ -15,6 +15,7 @@
 // Operands with k contiguous and operands stored [k][x] (W in dx, both in dW) use the same loop: the second kind is
 // read from LDS with the transposing 64-bit read. Global loads run three K-steps ahead in registers.
 #include "q8.h"
+#include <stdlib.h>
 #include "../../include/octsam.h"
 
 namespace {
@@ -41,17 +42,26 @@ __device__ __forceinline__ f32x4 mma(typename Elem<TY>::v8 a, typename Elem<TY>:
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// act(g) and, with GRAD, act'(g)
+// act(g) and, with GRAD, act'(g). The reciprocal is the hardware's (1 fp32 step). GELU's distribution function: 1 - q
+// or q with q = P(t) t exp(-g^2 / 2) / 2, t = 1 / (1 + 0.3275911 |g| / sqrt 2) (Abramowitz & Stegun 7.1.26, |error| of
+// 2 q <= 1.5e-7), so that the left tail keeps its relative precision
 template <bool GRAD>
 __device__ __forceinline__ float act_value(int act, float g, float& slope) {
   if (act == OCT_SILU) {
-    const float p = 1.0f / (1.0f + __expf(-g));
+    const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
     if constexpr (GRAD) slope = p * fmaf(g, 1.0f - p, 1.0f);
     return g * p;
   }
   if (act == OCT_GELU) {
-    const float cdf = 0.5f * (1.0f + erf_fast(g * 0.70710678118654752f));
-    if constexpr (GRAD) slope = fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), cdf);
+    using namespace gelu_c;
+    const float t = __builtin_amdgcn_rcpf(fmaf(P, fabsf(g), 1.0f));
+    float c = fmaf(t, A5, A4);
+    c = fmaf(c, t, A3);
+    c = fmaf(c, t, A2);
+    c = fmaf(c, t, A1);
+    const float ex = __builtin_amdgcn_exp2f(g * E * g), q = c * t * ex;
+    const float cdf = g < 0.0f ? q : 1.0f - q;
+    if constexpr (GRAD) slope = fmaf(g * 0.3989422804014327f, ex, cdf);
     return g * cdf;
   }
   if (act == OCT_RELU) {
@@ -75,33 +85,55 @@ __device__ __forceinline__ void row8(f32x4 a, f32x4 b, float* v) {
   }
 }
 
+// the largest of v over the four lanes (16 apart) that hold an 8-bit group
+__device__ __forceinline__ float group_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+// amax ignores NaN; only where it is infinite are the finite values searched again
 __device__ __forceinline__ void keep8_q(const GatedP& p, long long m, int half, int f, bool ok, const float* v) {
   float a = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) a = fmaxf(a, ok ? finite_abs(v[e]) : 0.0f);
-  a = fmaxf(a, __shfl_xor(a, 16, 64));
-  a = fmaxf(a, __shfl_xor(a, 32, 64));
+  for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e]));
+  a = group_max(ok ? a : 0.0f);
+  const bool inf = !is_finite(a);
+  if (__any(inf)) {
+    float b = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b = fmaxf(b, finite_abs(v[e]));
+    b = group_max(ok ? b : 0.0f);
+    if (inf) a = b;
+  }
   if (ok) {
     const int b = q8_scale(a);
     const float inv = q8_inverse(b);
-    *(u32x2*)((uint8_t*)p.save + m * p.ldsave + (long long)half * p.N + f) = (u32x2){q8_pack4(v, inv), q8_pack4(v + 4, inv)};
+    *(u32x2*)((uint8_t*)p.save + m * p.ldsave + (long long)half * p.N + f) =
+        inf ? (u32x2){q8_pack4(v, inv), q8_pack4(v + 4, inv)} : (u32x2){q8_pack4_plain(v, inv), q8_pack4_plain(v + 4, inv)};
     if ((f & 31) == 0) p.scale[m * p.ldscale + half * ((p.N + 31) / 32) + (f >> 5)] = (uint8_t)b;
   }
+}
+
+struct Bias8 {
+  float g[8], u[8];
+};
+__device__ __forceinline__ Bias8 load_bias(const GatedP& p, int f) {
+  Bias8 b = {};
+  if (p.bias && f < p.N) {
+    load8<T_F32>(p.bias, f, b.g);
+    load8<T_F32>(p.bias, (long long)p.N + f, b.u);
+  }
+  return b;
 }
 
 // g, u: a lane's 8 features from f on of row m (all lanes of a wave call this together). Rows past M and features
 // past F (a multiple of 8) are dropped; f % 32 is the same in the four lanes that hold an 8-bit group
 template <int TY>
-__device__ __forceinline__ void gated_store(const GatedP& p, long long m, int f, float* g, float* u) {
+__device__ __forceinline__ void gated_store(const GatedP& p, long long m, int f, const Bias8& b, float* g, float* u) {
   const bool ok = m < p.M && f < p.N;
-  if (p.bias && ok) {
-    float b[8];
-    load8<T_F32>(p.bias, f, b);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] += b[e];
-    load8<T_F32>(p.bias, (long long)p.N + f, b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] += b[e];
+  for (int e = 0; e < 8; ++e) {
+    g[e] += b.g[e];
+    u[e] += b.u[e];
   }
   if (p.save_type == T_Q8) {
     keep8_q(p, m, 0, f, ok, g);
@@ -110,12 +142,18 @@ __device__ __forceinline__ void gated_store(const GatedP& p, long long m, int f,
     store8<TY>(p.save, m * p.ldsave + f, g);
     store8<TY>(p.save, m * p.ldsave + p.N + f, u);
   }
-  if (ok) {
-    float h[8], unused;
+  float h[8], unused;
+  if (p.act == OCT_SILU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = act_value<false>(OCT_SILU, g[e], unused) * u[e];
+  } else if (p.act == OCT_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = act_value<false>(OCT_GELU, g[e], unused) * u[e];
+  } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[e] = act_value<false>(p.act, g[e], unused) * u[e];
-    store8<TY>(p.C, m * p.ldc + f, h);
   }
+  if (ok) store8<TY>(p.C, m * p.ldc + f, h);
 }
 
 template <int TY>
@@ -233,11 +271,228 @@ __global__ __launch_bounds__(256) void gated_tile_kernel(GatedP p, int tiles_n) 
   row8(acc[0], acc[1], v0);
   row8(acc[2], acc[3], v1);
   if constexpr (MODE == GATED) {
-    gated_store<TY>(p, m, col0 + cofs, v0, v1);
+    gated_store<TY>(p, m, col0 + cofs, load_bias(p, col0 + cofs), v0, v1);
   } else {
     plain_store<TY>(p, m, col0 + cofs, blockIdx.y, v0);
     plain_store<TY>(p, m, col0 + 32 + cofs, blockIdx.y, v1);
   }
+}
+
+// ----------------------------------------------------------------------------------------------------- 256 x 256 tile
+// Large products: 256 x 256 x 64 tiles (GATED: 128 features, gate and up rows in turns of 32), eight waves as 2 (rows)
+// x 4 (columns) with 128 x 64 each, operands by LDS-DMA through buffer descriptors (what lies past an operand's end
+// reads as zero), two stages of 64 KiB. A K-step of a wave is two segments between barriers: L reads its 24 fragments
+// and issues its share of the DMA, C runs its 64 MFMAs; the two wave rows run one segment apart, so that each SIMD has
+// one wave in its MFMAs while its other wave loads. A's rows 0-127 are read by wave row 0 alone (segment 2t), 128-255
+// by wave row 1 (2t + 1), B by both, and a region is refilled once its last reader has passed a barrier:
+//   wave row 0 in L(t): B(t + 1), landed at the end of its C(t)
+//   wave row 1 in L(t): A-hi(t + 1), landed at the end of its C(t); A-lo(t + 2), landed at the end of its L(t + 1)
+//   before the loop:    stage 0 and A-lo(1)
+// LDS images: rows of k as above; [k][x] operands as two halves of 128 columns, [64][256 B], chunk c of row r at
+// c ^ 2 ((r & 3) << 1 | (r >> 3) & 1): a transposing read's 32 lanes (rows q of 4, and 8 + q) cover 16 chunk slots, and
+// a fragment's address is one xor of a lane constant with the column block, plus constants.
+constexpr int STAGE = 65536, OUT_OF_RANGE = (int)0x80000000;
+
+__device__ __forceinline__ void hard_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void* base, long long bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)(bytes > 0 ? bytes : 0), 0x00020000);
+}
+
+template <int TY, bool KM>
+__device__ __forceinline__ typename Elem<TY>::v8 frag256(const char* img, int x0, int kb, int lane) {
+  typedef typename Elem<TY>::v8 v8;
+  if constexpr (!KM) {
+    return *(const v8*)(img + kc_at(x0 + (lane & 15), kb * 4 + (lane >> 4)));
+  } else {  // img: the 128-column half, x0 < 128
+    const int g = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
+    const int base = (8 * g + q) * 256 + (((q << 1) | (g & 1)) << 5) + ((pp >> 1) << 4) + 8 * (pp & 1);
+    const char* at = img + (base ^ (x0 << 1)) + kb * 8192;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 1024));
+    const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(v8, v);
+  }
+}
+
+// acc = the tile at (row0, col0) over the K-steps [kb, kb + n), n >= 1
+template <int TY, int MODE>
+__device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col0, int kb, int n, f32x4 (&acc)[8][4], char* lds,
+                                        int wave, int lane) {
+  typedef typename Elem<TY>::v8 v8;
+  constexpr bool AKM = MODE == TN, BKM = MODE != GATED;
+  const int wr = wave >> 2, wc = wave & 3;
+  const long long lda2 = p.lda * 2, ldb2 = p.ldb * 2;
+  const char *A = (const char*)p.A, *B = (const char*)p.B;
+  // a lane's part of a 1 KiB DMA piece j. k in rows: 8 rows of 128 B, by j & 1; [k][x]: 4 rows of 256 B, by (j >> 1) & 1
+  // (the part of the chunk swizzle that the piece number gives)
+  int va[2], vb[2];
+  auto lane_part = [&](bool km, int e, long long ld2) {
+    if (km) return (int)((lane >> 4) * ld2) + (((lane & 15) ^ (((lane >> 4) << 2) | (e << 1))) << 4);
+    const int r = e * 8 + (lane >> 3);
+    return (int)(r * ld2) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
+  };
+#pragma unroll
+  for (int e = 0; e < 2; ++e) va[e] = lane_part(AKM, e, lda2);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) vb[e] = lane_part(BKM, e, ldb2);
+  const __amdgpu_buffer_rsrc_t ra = range(A + row0 * lda2, (p.M - row0 < 256 ? p.M - row0 : 256) * lda2);
+  const int nf = p.N - col0 < 128 ? p.N - col0 : 128;
+  const __amdgpu_buffer_rsrc_t rg = range(B + (long long)col0 * ldb2, nf * ldb2);
+  const __amdgpu_buffer_rsrc_t ru = range(B + ((long long)p.N + col0) * ldb2, nf * ldb2);
+  // 16-B chunk of a row of k that lies past K (only in the last K-step of a K that is no multiple of 64)
+  auto cut = [&](int v, int e, int t) {
+    const int r = e * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+    return (kb + t) * 64 + 64 <= p.K || (kb + t) * 64 + c * 8 < p.K ? v : OUT_OF_RANGE;
+  };
+  auto km_range = [&](const char* X, long long ld2, long long x0, long long xdim, int t) {
+    const long long k = (long long)(kb + t) * 64, rows = p.K - k < 64 ? p.K - k : 64;
+    return range(X + k * ld2 + x0 * 2, (rows - 1) * ld2 + (xdim - x0) * 2);
+  };
+  auto dma_a = [&](int h, int j, int t) {  // piece j (of 16) of A's half h, stage t
+    const lds_ptr_t dst = (lds_ptr_t)(lds + (t & 1) * STAGE + h * 16384 + j * 1024);
+    if constexpr (AKM)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(km_range(A, lda2, row0 + h * 128, p.M, t), dst, 16, va[(j >> 1) & 1], (int)(4 * j * lda2), 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, dst, 16, cut(va[j & 1], j & 1, t),
+                                               (int)((h * 128 + (j & ~1) * 8) * lda2) + (kb + t) * 128, 0, 0);
+  };
+  auto dma_b = [&](int j, int t) {  // piece j (of 32) of B, stage t
+    const lds_ptr_t dst = (lds_ptr_t)(lds + (t & 1) * STAGE + 32768 + j * 1024);
+    if constexpr (BKM) {
+      const int h = j >> 4, jj = j & 15;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(km_range(B, ldb2, col0 + h * 128, p.N, t), dst, 16, vb[(jj >> 1) & 1], (int)(4 * jj * ldb2), 0, 0);
+    } else {
+      const int jj = j & 7;  // image rows 64 w + (0-31: gate features 32 w .., 32-63: the same features' up rows)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(jj < 4 ? rg : ru, dst, 16, cut(vb[j & 1], j & 1, t),
+                                               (int)(((j >> 3) * 32 + (jj & 2) * 8) * ldb2) + (kb + t) * 128, 0, 0);
+    }
+  };
+#pragma unroll
+  for (int mi = 0; mi < 8; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4)0.0f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) dma_a(0, wave * 2 + i, 0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) dma_a(1, wave * 2 + i, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dma_b(wave * 4 + i, 0);
+  if (n > 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) dma_a(0, wave * 2 + i, 1);
+    wait_loads<2>();
+  } else {
+    wait_loads<0>();
+  }
+  hard_barrier();
+  if (wr == 1) hard_barrier();
+  for (int t = 0; t < n; ++t) {
+    const char* cur = lds + (t & 1) * STAGE;
+    v8 af[8][2], bf[4][2];
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh) {
+#pragma unroll
+      for (int ni = 0; ni < 4; ++ni) {
+        if constexpr (BKM) bf[ni][kh] = frag256<TY, true>(cur + 32768 + (wc >> 1) * 16384, (wc & 1) * 64 + ni * 16, kh, lane);
+        else bf[ni][kh] = frag256<TY, false>(cur + 32768, wc * 64 + ni * 16, kh, lane);
+      }
+#pragma unroll
+      for (int mi = 0; mi < 8; ++mi) {
+        if constexpr (AKM) af[mi][kh] = frag256<TY, true>(cur + wr * 16384, mi * 16, kh, lane);
+        else af[mi][kh] = frag256<TY, false>(cur, wr * 128 + mi * 16, kh, lane);
+      }
+    }
+    if (wr == 0) {
+      if (t + 1 < n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dma_b(wc * 8 + i, t + 1);
+      }
+    } else {
+      if (t + 1 < n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dma_a(1, wc * 4 + i, t + 1);
+      }
+      if (t + 2 < n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dma_a(0, wc * 4 + i, t + 2);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the fragments are in registers: the stage may be refilled)
+    if (wr == 1) {
+      if (t + 2 < n) wait_loads<8>();
+      else if (t + 1 < n) wait_loads<4>();
+      else wait_loads<0>();
+    }
+    hard_barrier();
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int mi = 0; mi < 8; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = mma<TY>(bf[ni][kh], af[mi][kh], acc[mi][ni]);
+    if (wr == 0) {
+      wait_loads<0>();
+      hard_barrier();
+    } else {
+      if (t + 2 < n) wait_loads<4>();
+      else wait_loads<0>();
+      if (t + 1 < n) hard_barrier();
+    }
+  }
+}
+
+template <int TY, int MODE>
+__device__ __forceinline__ void store256(const GatedP& p, long long row0, int col0, f32x4 (&acc)[8][4], int wave, int lane) {
+  const int wr = wave >> 2, wc = wave & 3, q = lane >> 4, cofs = 16 * (q & 1) + 8 * (q >> 1);
+  Bias8 b;
+  if constexpr (MODE == GATED) b = load_bias(p, col0 + wc * 32 + cofs);
+#pragma unroll
+  for (int mi = 0; mi < 8; ++mi) {
+    const long long m = row0 + wr * 128 + mi * 16 + (lane & 15);
+    float v0[8], v1[8];
+    row8(acc[mi][0], acc[mi][1], v0);
+    row8(acc[mi][2], acc[mi][3], v1);
+    if constexpr (MODE == GATED) {
+      gated_store<TY>(p, m, col0 + wc * 32 + cofs, b, v0, v1);
+    } else {
+      plain_store<TY>(p, m, col0 + wc * 64 + cofs, 0, v0);
+      plain_store<TY>(p, m, col0 + wc * 64 + 32 + cofs, 0, v1);
+    }
+  }
+}
+
+// tiles go to the XCDs (workgroup id mod 8) in contiguous runs, and within a run eight row tiles take turns over the
+// column tiles, so that the 32 tiles in flight on an XCD share 8 row panels and 4 column panels in its L2
+__device__ __forceinline__ int tile_of(int bid, int nwg) {
+  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, loc = bid >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + loc;
+}
+__device__ __forceinline__ void place(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int per = 8 * tiles_n, g = id / per, in = id - g * per;
+  const int h = tiles_m - g * 8 < 8 ? tiles_m - g * 8 : 8;
+  tn = in / h;
+  tm = g * 8 + (in - tn * h);
+}
+
+template <int TY, int MODE>
+__global__ __launch_bounds__(512, 2) void gated_big_kernel(GatedP p, int tiles_m, int tiles_n) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tm, tn;
+  place(tile_of(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
+  const long long row0 = (long long)tm * 256;
+  const int col0 = tn * (MODE == GATED ? 128 : 256);
+  f32x4 acc[8][4];
+  tile256<TY, MODE>(p, row0, col0, 0, (p.K + 63) / 64, acc, lds, wave, lane);
+  store256<TY, MODE>(p, row0, col0, acc, wave, lane);
 }
 
 // out = the sum of the K splits' fp32 partials in order, rounded once
@@ -341,7 +596,25 @@ int splits_for(long long tiles, long long K) {
 int kper_of(long long K, int splits) { return (int)(((K + 63) / 64 + splits - 1) / splits * 64); }
 
 template <int TY, int MODE>
+int product_big(const GatedP& p, hipStream_t s) {
+  const int tiles_m = (int)(((long long)p.M + 255) / 256), per = MODE == GATED ? 128 : 256, tiles_n = (p.N + per - 1) / per;
+  (void)hipFuncSetAttribute((const void*)gated_big_kernel<TY, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * STAGE);
+  hipLaunchKernelGGL((gated_big_kernel<TY, MODE>), dim3((unsigned)((long long)tiles_m * tiles_n)), dim3(512), 2 * STAGE, s, p,
+                     tiles_m, tiles_n);
+  return 0;
+}
+int big_from() {  // TEMP tuning
+  static const int v = getenv("GATED_BIG") ? atoi(getenv("GATED_BIG")) : 128;
+  return v;
+}
+
+template <int TY, int MODE>
 int product(GatedP p, void* ws, hipStream_t s) {
+  {
+    const int per = MODE == GATED ? 128 : 256;
+    const long long t = (((long long)p.M + 255) / 256) * ((p.N + per - 1) / per);
+    if (t >= big_from() && p.K > 0 && p.lda < (1 << 21) && p.ldb < (1 << 21)) return product_big<TY, MODE>(p, s);
+  }
   const long long tiles_m = ((long long)p.M + 63) / 64, tiles_n = MODE == GATED ? ((long long)p.N + 31) / 32 : ((long long)p.N + 63) / 64;
   const long long tiles = tiles_m * tiles_n;
   OCTSAM_CHECK_ARG(tiles < (1ll << 31), "gated: too many tiles");

@@ -44,6 +44,13 @@ __device__ __forceinline__ uint32_t q8_pack4(const float* x, float inv) {
   r = __builtin_amdgcn_cvt_pk_fp8_f32(q8_ready(x[2], inv), q8_ready(x[3], inv), r, true);
   return (uint32_t)r;
 }
+// the same for values known to be finite or NaN (a NaN's product is NaN)
+__device__ __forceinline__ uint32_t q8_pack4_plain(const float* x, float inv) {
+  int r = 0;
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, r, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, r, true);
+  return (uint32_t)r;
+}
 __device__ __forceinline__ uint8_t q8_pack1(float x, float inv) {
   return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(q8_ready(x, inv), 0.0f, 0, false) & 0xff);
 }
