@@ -482,17 +482,92 @@ __device__ __forceinline__ void place(int id, int tiles_m, int tiles_n, int& tm,
   tm = g * 8 + (in - tn * h);
 }
 
+// How a product's tiles meet the chip's 256 workgroups: `whole` tiles (a multiple of 256) are one workgroup's each. Of
+// the `rest` others K is cut into `splits` parts, all tiles at the same places; of the rest * splits parts, in the order
+// part-major, the first `wgs` are a workgroup's first job each, so that what runs together on an XCD walks the same K
+// over neighbouring tiles and shares its panels in L2 (cut end to end into equal runs instead, every workgroup walked a
+// K of its own: dw of 16384 x 1280 x 3416 353 us, against 230). What is left, `over` tiles' last parts, is laid end to
+// end and cut into wgs equal runs, the second jobs, each in at most two tiles. All jobs leave fp32 partial tiles (slot w,
+// then wgs + 2 w and wgs + 2 w + 1), and gated_fix_kernel adds a tile's in order. wgs = 0: every tile is whole.
+struct Share {
+  int tiles_m, tiles_n, steps, whole, rest, splits, wgs, over;
+};
+__device__ __host__ __forceinline__ int part_start(const Share& s, int j) { return (int)((long long)j * s.steps / s.splits); }
+__device__ __host__ __forceinline__ int last_part(const Share& s) { return s.steps - part_start(s, s.splits - 1); }
+__device__ __host__ __forceinline__ int run_start(const Share& s, int w) { return (int)((long long)w * s.over * last_part(s) / s.wgs); }
+
 template <int TY, int MODE>
-__global__ __launch_bounds__(512, 2) void gated_big_kernel(GatedP p, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(512, 2) void gated_big_kernel(GatedP p, Share sh, float* part) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int tm, tn;
-  place(tile_of(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
-  const long long row0 = (long long)tm * 256;
-  const int col0 = tn * (MODE == GATED ? 128 : 256);
   f32x4 acc[8][4];
-  tile256<TY, MODE>(p, row0, col0, 0, (p.K + 63) / 64, acc, lds, wave, lane);
-  store256<TY, MODE>(p, row0, col0, acc, wave, lane);
+  int tm, tn;
+  if (MODE == GATED || (int)blockIdx.x < sh.whole) {
+    place(tile_of(blockIdx.x, MODE == GATED ? gridDim.x : sh.whole), sh.tiles_m, sh.tiles_n, tm, tn);
+    const long long row0 = (long long)tm * 256;
+    const int col0 = tn * (MODE == GATED ? 128 : 256);
+    tile256<TY, MODE>(p, row0, col0, 0, sh.steps, acc, lds, wave, lane);
+    store256<TY, MODE>(p, row0, col0, acc, wave, lane);
+    return;
+  }
+  if constexpr (MODE != GATED) {
+    const int w = tile_of(blockIdx.x - sh.whole, sh.wgs);
+    auto job = [&](int t, int kb, int n, int slot) {
+      place(sh.whole + t, sh.tiles_m, sh.tiles_n, tm, tn);
+      tile256<TY, MODE>(p, (long long)tm * 256, tn * 256, kb, n, acc, lds, wave, lane);
+      GatedP q = p;
+      q.C = part + (long long)slot * 65536;
+      q.ldc = 256;
+      q.c_type = T_F32;
+      q.M = q.N = 256;
+      store256<TY, MODE>(q, 0, 0, acc, wave, lane);
+    };
+    const int end = run_start(sh, w + 1), len = last_part(sh), k_last = part_start(sh, sh.splits - 1);
+    int u = run_start(sh, w);
+    const int j0 = w / sh.rest;
+    int t = w - j0 * sh.rest, kb = part_start(sh, j0), n = part_start(sh, j0 + 1) - kb, slot = w;
+    for (int k = 0;; ++k) {
+      job(t, kb, n, slot);
+      if (u >= end) break;
+      const int l = u / len, in = u - l * len;
+      t = sh.rest - sh.over + l;
+      kb = k_last + in;
+      n = end - u < len - in ? end - u : len - in;
+      slot = sh.wgs + 2 * w + k;
+      u += n;
+    }
+  }
+}
+
+// the tiles that were left in partials: workgroup (8 rows, tile)
+template <int TY>
+__global__ __launch_bounds__(256) void gated_fix_kernel(GatedP p, Share sh, const float* __restrict__ part) {
+  const int t = blockIdx.y, r = blockIdx.x * 8 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 8;
+  int tm, tn;
+  place(sh.whole + t, sh.tiles_m, sh.tiles_n, tm, tn);
+  const long long m = (long long)tm * 256 + r;
+  const int n = tn * 256 + c;
+  if (m >= p.M || n >= p.N) return;
+  float v[8] = {};
+  auto add = [&](int slot) {
+    float x[8];
+    load8<T_F32>(part, (long long)slot * 65536 + r * 256 + c, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += x[e];
+  };
+  const int l = t - (sh.rest - sh.over);  // >= 0: the last part was shared out over runs
+  const int mains = l < 0 ? sh.splits : sh.splits - 1;
+  for (int j = 0; j < mains; ++j) add(j * sh.rest + t);
+  if (l >= 0) {
+    const long long len = last_part(sh), a = l * len, b = a + len, units = sh.over * len;
+    const int w0 = (int)(((a + 1) * sh.wgs - 1) / units), w1 = (int)((b * sh.wgs - 1) / units);  // runs of units a and b - 1
+    for (int w = w0; w <= w1; ++w) {
+      const int u = run_start(sh, w);
+      if (u < run_start(sh, w + 1)) add(sh.wgs + 2 * w + (u < a));
+    }
+  }
+  if (p.c_type == T_F32) store8<T_F32>(p.C, m * p.ldc + n, v);
+  else store8<TY>(p.C, m * p.ldc + n, v);
 }
 
 // out = the sum of the K splits' fp32 partials in order, rounded once
@@ -595,26 +670,55 @@ int splits_for(long long tiles, long long K) {
 }
 int kper_of(long long K, int splits) { return (int)(((K + 63) / 64 + splits - 1) / splits * 64); }
 
-template <int TY, int MODE>
-int product_big(const GatedP& p, hipStream_t s) {
-  const int tiles_m = (int)(((long long)p.M + 255) / 256), per = MODE == GATED ? 128 : 256, tiles_n = (p.N + per - 1) / per;
-  (void)hipFuncSetAttribute((const void*)gated_big_kernel<TY, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * STAGE);
-  hipLaunchKernelGGL((gated_big_kernel<TY, MODE>), dim3((unsigned)((long long)tiles_m * tiles_n)), dim3(512), 2 * STAGE, s, p,
-                     tiles_m, tiles_n);
-  return 0;
-}
-int big_from() {  // TEMP tuning
-  static const int v = getenv("GATED_BIG") ? atoi(getenv("GATED_BIG")) : 128;
-  return v;
+// shares a product of 256 x 256 tiles out; sharing costs about 10 K-steps (16 us: second jobs and the adding)
+Share share_out(Mode mode, long long M, long long N, long long K) {
+  Share s = {};
+  const int per = mode == GATED ? 128 : 256;
+  s.tiles_m = (int)((M + 255) / 256);
+  s.tiles_n = (int)((N + per - 1) / per);
+  s.steps = (int)((K + 63) / 64);
+  const long long tiles = (long long)s.tiles_m * s.tiles_n;
+  s.rest = (int)(tiles % 256);
+  s.whole = (int)tiles;
+  s.splits = 1;
+  if (mode == GATED || s.rest == 0 || s.steps < 8) return s;
+  int splits = (256 + s.rest - 1) / s.rest, over = 0;
+  if (splits > s.steps / 4) splits = s.steps / 4;
+  int wgs = s.rest * splits;
+  if (wgs > 256) {
+    over = wgs - 256;
+    wgs = 256;
+  }
+  s.splits = splits;
+  const double shared = (double)s.steps / splits + (double)over * last_part(s) / wgs + 10;
+  if (splits < 2 || shared > s.steps) {
+    s.splits = 1;
+    return s;
+  }
+  s.whole = (int)(tiles - s.rest);
+  s.wgs = wgs;
+  s.over = over;
+  return s;
 }
 
 template <int TY, int MODE>
+int product_big(const GatedP& p, const Share& sh, void* ws, hipStream_t s) {
+  (void)hipFuncSetAttribute((const void*)gated_big_kernel<TY, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * STAGE);
+  hipLaunchKernelGGL((gated_big_kernel<TY, MODE>), dim3((unsigned)(sh.whole + sh.wgs)), dim3(512), 2 * STAGE, s, p, sh, (float*)ws);
+  if (sh.wgs)
+    hipLaunchKernelGGL((gated_fix_kernel<TY>), dim3(32, (unsigned)sh.rest), dim3(256), 0, s, p, sh, (const float*)ws);
+  return 0;
+}
+int big_from() {  // TEMP tuning
+  static const int v = getenv("GATED_BIG") ? atoi(getenv("GATED_BIG")) : 64;
+  return v;
+}
+bool use_big(const Share& s) { return (long long)s.tiles_m * s.tiles_n >= big_from() && s.steps > 0; }
+
+template <int TY, int MODE>
 int product(GatedP p, void* ws, hipStream_t s) {
-  {
-    const int per = MODE == GATED ? 128 : 256;
-    const long long t = (((long long)p.M + 255) / 256) * ((p.N + per - 1) / per);
-    if (t >= big_from() && p.K > 0 && p.lda < (1 << 21) && p.ldb < (1 << 21)) return product_big<TY, MODE>(p, s);
-  }
+  const Share sh = share_out((Mode)MODE, p.M, p.N, p.K);
+  if (use_big(sh) && p.lda < (1 << 21) && p.ldb < (1 << 21)) return product_big<TY, MODE>(p, sh, ws, s);
   const long long tiles_m = ((long long)p.M + 63) / 64, tiles_n = MODE == GATED ? ((long long)p.N + 31) / 32 : ((long long)p.N + 63) / 64;
   const long long tiles = tiles_m * tiles_n;
   OCTSAM_CHECK_ARG(tiles < (1ll << 31), "gated: too many tiles");
@@ -648,10 +752,13 @@ int product(GatedP p, void* ws, hipStream_t s) {
 }
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
-int64_t join_bytes(int64_t M, int64_t N, int64_t K) {
+int64_t join_bytes(Mode mode, int64_t M, int64_t N, int64_t K) {  // of either kernel (the choice looks at strides too)
   if (M <= 0 || N <= 0) return 0;
+  const Share sh = share_out(mode, M, N, K);
+  const int64_t big = (int64_t)sh.wgs * (sh.over ? 3 : 1) * 65536 * 4;
   const int s = splits_for(((M + 63) / 64) * ((N + 63) / 64), K);
-  return s > 1 ? s * M * N * 4 : 0;
+  const int64_t small = s > 1 ? s * M * N * 4 : 0;
+  return big > small ? big : small;
 }
 // rows per workgroup of the element-wise backward (grid y: at most 32768 workgroups)
 int64_t slab_of(int64_t M) {
@@ -676,7 +783,7 @@ BwdPlan bwd_plan(int64_t M, int64_t D, int64_t F, bool x_q8) {
   b.part = at;
   at += round16((int64_t)b.slabs * 2 * F * 4);
   b.join = at;
-  const int64_t j1 = join_bytes(M, D, 2 * F), j2 = join_bytes(2 * F, D, M);
+  const int64_t j1 = join_bytes(NN, M, D, 2 * F), j2 = join_bytes(TN, 2 * F, D, M);
   at += round16(j1 > j2 ? j1 : j2);
   b.total = at;
   return b;
