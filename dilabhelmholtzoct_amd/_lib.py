@@ -217,14 +217,28 @@ def check(rc: int, what: str) -> None:
 
 
 def stream_handle(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of device (default: the current device), without the cost of a Stream object."""
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def call(name: str, *args) -> None:
     """Call a C-ABI entry point whose last argument is the stream; raise on error."""
-    fn = getattr(load(), name)
-    rc = fn(*args, c_void_p(stream_handle()))
-    check(rc, name)
+    rc = getattr(_lib or load(), name)(*args, stream_handle())
+    if rc:
+        check(rc, name)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """call() on device's current stream, whichever device is current (a launch goes to the current device)."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = getattr(_lib or load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            check(rc, name)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -191,17 +191,19 @@ __device__ __forceinline__ typename Elem<TY>::v8 frag64(const char* img, int x0,
   }
 }
 
+typedef char TileLds[2][2][64 * 128];  // [stage][operand]
+
+// tile `tile` (column tiles first) of K split `split`
 template <int TY, int MODE>
-__global__ __launch_bounds__(256) void gated_tile_kernel(GatedP p, int tiles_n) {
+__device__ __forceinline__ void tile64(const GatedP& p, int tiles_n, int tile, int split, TileLds& smem) {
   typedef typename Elem<TY>::v8 v8;
   constexpr bool AKM = MODE == TN, BKM = MODE != GATED;
-  constexpr int AHEAD = 3, IMG = 64 * 128;
-  __shared__ __attribute__((aligned(16))) char smem[2][2][IMG];
+  constexpr int AHEAD = 3;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
+  const int tm = tile / tiles_n, tn = tile - tm * tiles_n;
   const long long row0 = (long long)tm * 64;
   const int col0 = tn * (MODE == GATED ? 32 : 64);
-  const long long k0 = (long long)blockIdx.y * p.kper;
+  const long long k0 = (long long)split * p.kper;
   const int kn = (int)(p.K - k0 < p.kper ? p.K - k0 : p.kper);  // (< 1: no steps, the tile is zero)
   const int steps = kn > 0 ? (kn + 63) / 64 : 0;
 
@@ -273,8 +275,31 @@ __global__ __launch_bounds__(256) void gated_tile_kernel(GatedP p, int tiles_n) 
   if constexpr (MODE == GATED) {
     gated_store<TY>(p, m, col0 + cofs, load_bias(p, col0 + cofs), v0, v1);
   } else {
-    plain_store<TY>(p, m, col0 + cofs, blockIdx.y, v0);
-    plain_store<TY>(p, m, col0 + 32 + cofs, blockIdx.y, v1);
+    plain_store<TY>(p, m, col0 + cofs, split, v0);
+    plain_store<TY>(p, m, col0 + 32 + cofs, split, v1);
+  }
+}
+
+template <int TY>
+__global__ __launch_bounds__(256) void gated_tile_kernel(GatedP p, int tiles_n) {
+  __shared__ __attribute__((aligned(16))) TileLds smem;
+  tile64<TY, GATED>(p, tiles_n, blockIdx.x, 0, smem);
+}
+
+// both products of the backward in one launch: dx's tiles (each K split of all tiles in turn), then dw's
+struct TileJob {
+  GatedP p;
+  int tiles, tiles_n, splits;
+};
+template <int TY>
+__global__ __launch_bounds__(256) void gated_pair_kernel(TileJob x, TileJob w) {
+  __shared__ __attribute__((aligned(16))) TileLds smem;
+  int b = blockIdx.x;
+  if (b < x.tiles * x.splits) {
+    tile64<TY, NN>(x.p, x.tiles_n, b % x.tiles, b / x.tiles, smem);
+  } else {
+    b -= x.tiles * x.splits;
+    tile64<TY, TN>(w.p, w.tiles_n, b % w.tiles, b / w.tiles, smem);
   }
 }
 
@@ -557,7 +582,17 @@ __global__ __launch_bounds__(256) void gated_fix_kernel(GatedP p, Share sh, cons
   };
   const int l = t - (sh.rest - sh.over);  // >= 0: the last part was shared out over runs
   const int mains = l < 0 ? sh.splits : sh.splits - 1;
-  for (int j = 0; j < mains; ++j) add(j * sh.rest + t);
+  int j = 0;
+  for (; j + 4 <= mains; j += 4) {  // (four partials in flight)
+    float x[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load8<T_F32>(part, (long long)((j + i) * sh.rest + t) * 65536 + r * 256 + c, x[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += x[i][e];
+  }
+  for (; j < mains; ++j) add(j * sh.rest + t);
   if (l >= 0) {
     const long long len = last_part(sh), a = l * len, b = a + len, units = sh.over * len;
     const int w0 = (int)(((a + 1) * sh.wgs - 1) / units), w1 = (int)((b * sh.wgs - 1) / units);  // runs of units a and b - 1
@@ -570,21 +605,42 @@ __global__ __launch_bounds__(256) void gated_fix_kernel(GatedP p, Share sh, cons
   else store8<TY>(p.C, m * p.ldc + n, v);
 }
 
-// out = the sum of the K splits' fp32 partials in order, rounded once
+// What is left after the products, in one launch: the K splits' fp32 partials of dx and dw added in order and rounded
+// once (a thread: 8 columns), and the row slabs' partial sums of db (a workgroup: 32 columns).
+struct JoinJob {
+  const float* part;
+  void* out;
+  long long stride, rows, ldo;
+  int splits, nch, type;  // splits < 2: nothing to do
+  unsigned blocks;
+};
+struct DbJob {
+  const float* part;
+  float* out;
+  int slabs, n;
+  unsigned blocks;
+};
 template <int TY>
-__global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ part, long long stride, int splits,
-                                                         long long rows, int nch, void* __restrict__ out, long long ldo) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * nch) return;
-  const long long r = i / nch;
+__device__ __forceinline__ void join_block(const JoinJob& j, unsigned block) {
+  const long long i = (long long)block * 256 + threadIdx.x;
+  if (i >= j.rows * j.nch) return;
+  const long long r = i / j.nch;
   float v[8], t[8];
-  load8<T_F32>(part, i * 8, v);
-  for (int s = 1; s < splits; ++s) {
-    load8<T_F32>(part, s * stride + i * 8, t);
+  load8<T_F32>(j.part, i * 8, v);
+  for (int s = 1; s < j.splits; ++s) {
+    load8<T_F32>(j.part, s * j.stride + i * 8, t);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += t[e];
   }
-  store8<TY>(out, r * ldo + (i - r * nch) * 8, v);
+  const long long at = r * j.ldo + (i - r * j.nch) * 8;
+  if (j.type == T_F32) store8<T_F32>(j.out, at, v);
+  else store8<TY>(j.out, at, v);
+}
+template <int TY>
+__global__ __launch_bounds__(256) void gated_finish_kernel(JoinJob x, JoinJob w, DbJob d) {
+  if (blockIdx.x < x.blocks) return join_block<TY>(x, blockIdx.x);
+  if (blockIdx.x < x.blocks + w.blocks) return join_block<TY>(w, blockIdx.x - x.blocks);
+  column_sums(d.part, d.slabs, d.n, (blockIdx.x - x.blocks - w.blocks) * 32, d.out);
 }
 
 // --------------------------------------------------------------------------------------------- element-wise backward
@@ -596,13 +652,32 @@ struct ActBwd {
   long long lddh, ldgu, ldgs, lddgu, ldh, M;
   long long slab;
   int F, act;
+  const void* x8;  // an 8-bit x to be read back into x16 [M][D], or null
+  const uint8_t* xs;
+  void* x16;
+  long long ldx, ldxs;
+  int D;
 };
 
-// workgroup (x, y): 256 features (32 lanes of 8) of the rows [y * slab, (y + 1) * slab), eight rows at a time
+// workgroup (x, y): 256 features (32 lanes of 8) of the rows [y * slab, (y + 1) * slab), eight rows at a time; behind
+// the features' workgroups, those that read 256 columns of an 8-bit x back for dw's product
 template <int TY, int ST>
 __global__ __launch_bounds__(256) void gated_act_bwd_kernel(ActBwd a) {
   __shared__ float fold[8][16][33];
-  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5, feature_blocks = (a.F + 255) / 256;
+  if ((int)blockIdx.x >= feature_blocks) {
+    const int c = (blockIdx.x - feature_blocks) * 256 + lane * 8;
+    const long long r0 = (long long)blockIdx.y * a.slab, r1 = r0 + a.slab < a.M ? r0 + a.slab : a.M;
+    for (long long r = r0 + sub; r < r1 && c < a.D; r += 8) {
+      const u32x2 q = *(const u32x2*)((const uint8_t*)a.x8 + r * a.ldx + c);
+      const float k = q8_value(a.xs[r * a.ldxs + (c >> 5)]);
+      float v[8];
+      q8_unpack4(q[0], k, v);
+      q8_unpack4(q[1], k, v + 4);
+      store8<TY>(a.x16, r * a.D + c, v);
+    }
+    return;
+  }
   const int f = blockIdx.x * 256 + lane * 8;
   const bool on = f < a.F;
   float db[16];
@@ -655,20 +730,40 @@ __global__ __launch_bounds__(256) void gated_act_bwd_kernel(ActBwd a) {
   }
 }
 
-__global__ void gated_zero_kernel(float* p, long long n) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) p[i] = 0.0f;
-}
-
 // ------------------------------------------------------------------------------------------------------------- host
-// K splits of a product with `tiles` output tiles: enough workgroups for the chip's 256 CUs twice over, at least four
-// K-steps each
-int splits_for(long long tiles, long long K) {
-  const long long steps = (K + 63) / 64, want = (511 + tiles) / tiles, most = steps / 4;
-  const long long s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// A product on 64 x 64 tiles: K splits so that `tiles` (of all products of the launch) give the chip's 256 CUs three
+// workgroups each, at least four K-steps a split
+TileJob tile_job(const GatedP& p, long long tiles) {
+  TileJob j = {};
+  j.p = p;
+  j.tiles_n = (p.N + 63) / 64;
+  j.tiles = (int)(((long long)p.M + 63) / 64 * j.tiles_n);
+  const int steps = (p.K + 63) / 64;
+  long long s = tiles > 0 ? (767 + tiles) / tiles : 1;
+  if (s > steps / 4) s = steps / 4;
+  j.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  j.p.kper = (steps + j.splits - 1) / j.splits * 64;
+  return j;
 }
-int kper_of(long long K, int splits) { return (int)(((K + 63) / 64 + splits - 1) / splits * 64); }
+// its partials go to ws: what is left to do for the output that p names
+JoinJob join_job(TileJob& j, void* ws) {
+  JoinJob f = {};
+  if (j.splits < 2) return f;
+  GatedP& p = j.p;
+  f.out = p.C;
+  f.ldo = p.ldc;
+  f.type = p.c_type;
+  f.part = (const float*)ws;
+  f.stride = p.split_stride = (long long)p.M * p.N;
+  f.rows = p.M;
+  f.nch = p.N / 8;
+  f.splits = j.splits;
+  f.blocks = (unsigned)((f.rows * f.nch + 255) / 256);
+  p.C = ws;
+  p.ldc = p.N;
+  p.c_type = T_F32;
+  return f;
+}
 
 // shares a product of 256 x 256 tiles out; sharing costs about 10 K-steps (16 us: second jobs and the adding)
 Share share_out(Mode mode, long long M, long long N, long long K) {
@@ -713,53 +808,40 @@ int big_from() {  // TEMP tuning
   static const int v = getenv("GATED_BIG") ? atoi(getenv("GATED_BIG")) : 64;
   return v;
 }
+// operand strides up to which the 256 x 256 kernel's 32-bit offsets reach
+bool near(int64_t ld) { return ld < (1 << 21); }
 bool use_big(const Share& s) { return (long long)s.tiles_m * s.tiles_n >= big_from() && s.steps > 0; }
 
-template <int TY, int MODE>
-int product(GatedP p, void* ws, hipStream_t s) {
-  const Share sh = share_out((Mode)MODE, p.M, p.N, p.K);
-  if (use_big(sh) && p.lda < (1 << 21) && p.ldb < (1 << 21)) return product_big<TY, MODE>(p, sh, ws, s);
-  const long long tiles_m = ((long long)p.M + 63) / 64, tiles_n = MODE == GATED ? ((long long)p.N + 31) / 32 : ((long long)p.N + 63) / 64;
-  const long long tiles = tiles_m * tiles_n;
-  OCTSAM_CHECK_ARG(tiles < (1ll << 31), "gated: too many tiles");
-  if (MODE == GATED) {
-    p.kper = (p.K + 63) / 64 * 64;
-    hipLaunchKernelGGL((gated_tile_kernel<TY, MODE>), dim3((unsigned)tiles), dim3(256), 0, s, p, (int)tiles_n);
-    return 0;
-  }
-  const int splits = splits_for(tiles, p.K);
-  p.kper = kper_of(p.K, splits);
-  if (splits == 1) {
-    hipLaunchKernelGGL((gated_tile_kernel<TY, MODE>), dim3((unsigned)tiles), dim3(256), 0, s, p, (int)tiles_n);
-    return 0;
-  }
-  void* out = p.C;
-  const long long ldo = p.ldc;
-  const int out_type = p.c_type;
-  p.C = ws;
-  p.ldc = p.N;
-  p.c_type = T_F32;
-  p.split_stride = (long long)p.M * p.N;
-  hipLaunchKernelGGL((gated_tile_kernel<TY, MODE>), dim3((unsigned)tiles, splits), dim3(256), 0, s, p, (int)tiles_n);
-  const long long items = (long long)p.M * (p.N / 8);
-  if (out_type == T_F32)
-    hipLaunchKernelGGL((gated_join_kernel<T_F32>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, (const float*)ws,
-                       p.split_stride, splits, (long long)p.M, p.N / 8, out, ldo);
-  else
-    hipLaunchKernelGGL((gated_join_kernel<TY>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, (const float*)ws,
-                       p.split_stride, splits, (long long)p.M, p.N / 8, out, ldo);
+template <int TY>
+int forward(const GatedP& p, hipStream_t s) {
+  const Share sh = share_out(GATED, p.M, p.N, p.K);
+  if (use_big(sh) && near(p.lda) && near(p.ldb)) return product_big<TY, GATED>(p, sh, nullptr, s);
+  const int tiles_n = (p.N + 31) / 32;
+  const long long tiles = ((long long)p.M + 63) / 64 * tiles_n;
+  OCTSAM_CHECK_ARG(tiles < (1ll << 31), "gated_fwd: too many tiles");
+  GatedP q = p;
+  q.kper = (p.K + 63) / 64 * 64;
+  hipLaunchKernelGGL((gated_tile_kernel<TY>), dim3((unsigned)tiles), dim3(256), 0, s, q, tiles_n);
   return 0;
 }
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
-int64_t join_bytes(Mode mode, int64_t M, int64_t N, int64_t K) {  // of either kernel (the choice looks at strides too)
+int64_t tiles_of(int64_t M, int64_t N) { return ((M + 63) / 64) * ((N + 63) / 64); }
+// bytes of fp32 partials of a product: on 256 x 256 tiles, or (as strides far apart can ask for) on 64 x 64 tiles, of
+// which both products have `tiles`
+int64_t partial_bytes(Mode mode, int64_t M, int64_t N, int64_t K, int64_t tiles) {
   if (M <= 0 || N <= 0) return 0;
   const Share sh = share_out(mode, M, N, K);
   const int64_t big = (int64_t)sh.wgs * (sh.over ? 3 : 1) * 65536 * 4;
-  const int s = splits_for(((M + 63) / 64) * ((N + 63) / 64), K);
-  const int64_t small = s > 1 ? s * M * N * 4 : 0;
-  return big > small ? big : small;
+  GatedP p = {};
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  const int splits = tile_job(p, tiles).splits;
+  const int64_t small = splits > 1 ? splits * M * N * 4 : 0;
+  return round16(big > small ? big : small);
 }
+
 // rows per workgroup of the element-wise backward (grid y: at most 32768 workgroups)
 int64_t slab_of(int64_t M) {
   const int64_t least = (M + 32767) / 32768, want = M <= 64 ? 8 : M <= 2048 ? 32 : 64;
@@ -767,7 +849,7 @@ int64_t slab_of(int64_t M) {
 }
 
 struct BwdPlan {
-  int64_t dgu, x16, part, join, total;
+  int64_t dgu, x16, part, join_x, join_w, total;
   int64_t slab;
   int slabs;
 };
@@ -782,9 +864,11 @@ BwdPlan bwd_plan(int64_t M, int64_t D, int64_t F, bool x_q8) {
   at += x_q8 ? round16(M * D * 2) : 0;
   b.part = at;
   at += round16((int64_t)b.slabs * 2 * F * 4);
-  b.join = at;
-  const int64_t j1 = join_bytes(NN, M, D, 2 * F), j2 = join_bytes(TN, 2 * F, D, M);
-  at += round16(j1 > j2 ? j1 : j2);
+  b.join_x = at;
+  const int64_t tiles = tiles_of(M, D) + tiles_of(2 * F, D);
+  at += partial_bytes(NN, M, D, 2 * F, tiles);
+  b.join_w = at;
+  at += partial_bytes(TN, 2 * F, D, M, tiles);
   b.total = at;
   return b;
 }
@@ -794,40 +878,46 @@ constexpr int64_t MAX_M = 1ll << 30, MAX_W = 1 << 24;
 
 template <int TY>
 int run_bwd(const BwdPlan& b, const ActBwd& act, int gu_type, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
-            int D, int F, void* dx, int64_t lddx, void* dw, int dw_type, int64_t lddw, char* ws, hipStream_t s) {
+            int D, int F, void* dx, int64_t lddx, void* dw, int dw_type, int64_t lddw, float* db, char* ws, hipStream_t s) {
   if (M > 0) {
-    const dim3 grid((unsigned)((F + 255) / 256), (unsigned)b.slabs);
+    const dim3 grid((unsigned)((F + 255) / 256 + (act.x8 ? (D + 255) / 256 : 0)), (unsigned)b.slabs);
     if (gu_type == T_Q8) hipLaunchKernelGGL((gated_act_bwd_kernel<TY, T_Q8>), grid, dim3(256), 0, s, act);
     else hipLaunchKernelGGL((gated_act_bwd_kernel<TY, TY>), grid, dim3(256), 0, s, act);
   }
-  GatedP p = {};
-  p.save_type = T_NONE;
-  if (dx && M > 0) {
-    p.A = ws + b.dgu;
-    p.lda = 2 * (int64_t)F;
-    p.B = w;
-    p.ldb = ldw;
-    p.C = dx;
-    p.ldc = lddx;
-    p.c_type = TY;
-    p.M = (int)M;
-    p.N = D;
-    p.K = 2 * F;
-    if (int rc = product<TY, NN>(p, ws + b.join, s)) return rc;
+  GatedP px = {}, pw = {};
+  px.A = pw.A = ws + b.dgu;
+  px.lda = pw.lda = 2 * (int64_t)F;
+  px.save_type = pw.save_type = T_NONE;
+  px.N = pw.N = D;
+  px.B = w, px.ldb = ldw, px.C = dx, px.ldc = lddx, px.c_type = TY, px.M = (int)M, px.K = 2 * F;
+  pw.B = x, pw.ldb = ldx, pw.C = dw, pw.ldc = lddw, pw.c_type = dw_type, pw.M = 2 * F, pw.K = (int)M;
+  const Share shx = share_out(NN, M, D, 2 * F), shw = share_out(TN, 2 * F, D, M);
+  const bool big_x = use_big(shx) && near(px.lda) && near(ldw), big_w = use_big(shw) && near(pw.lda) && near(ldx);
+  if (dx && M > 0 && big_x)
+    if (int rc = product_big<TY, NN>(px, shx, ws + b.join_x, s)) return rc;
+  if (dw && big_w)
+    if (int rc = product_big<TY, TN>(pw, shw, ws + b.join_w, s)) return rc;
+  const bool tile_x = dx && M > 0 && !big_x, tile_w = dw && !big_w;
+  TileJob jx = {}, jw = {};
+  JoinJob fx = {}, fw = {};
+  if (tile_x || tile_w) {
+    const int64_t tiles = tiles_of(M, D) + tiles_of(2 * F, D);  // (whichever are asked for: the same bits)
+    OCTSAM_CHECK_ARG(tiles < (1 << 24), "gated_bwd: too many tiles");
+    if (tile_x) jx = tile_job(px, tiles), fx = join_job(jx, ws + b.join_x);
+    if (tile_w) jw = tile_job(pw, tiles), fw = join_job(jw, ws + b.join_w);
+    const int blocks = jx.tiles * jx.splits + jw.tiles * jw.splits;
+    hipLaunchKernelGGL((gated_pair_kernel<TY>), dim3((unsigned)blocks), dim3(256), 0, s, jx, jw);
   }
-  if (dw) {
-    p.A = ws + b.dgu;
-    p.lda = 2 * (int64_t)F;
-    p.B = x;
-    p.ldb = ldx;
-    p.C = dw;
-    p.ldc = lddw;
-    p.c_type = dw_type;
-    p.M = 2 * F;
-    p.N = D;
-    p.K = (int)M;
-    if (int rc = product<TY, TN>(p, ws + b.join, s)) return rc;
+  DbJob d = {};
+  if (db) {
+    d.part = (const float*)(ws + b.part);
+    d.out = db;
+    d.slabs = b.slabs;  // (none without rows: db is zero)
+    d.n = 2 * F;
+    d.blocks = (unsigned)((d.n + 31) / 32);
   }
+  if (const unsigned blocks = fx.blocks + fw.blocks + d.blocks)
+    hipLaunchKernelGGL((gated_finish_kernel<TY>), dim3(blocks), dim3(256), 0, s, fx, fw, d);
   return 0;
 }
 
@@ -868,8 +958,7 @@ extern "C" int octsam_gated_fwd(const void* x, int64_t ldx, const void* w, int64
   p.N = F;
   p.K = D;
   p.act = act;
-  const int rc = type == T_BF16 ? product<T_BF16, GATED>(p, nullptr, (hipStream_t)stream)
-                                : product<T_F16, GATED>(p, nullptr, (hipStream_t)stream);
+  const int rc = type == T_BF16 ? forward<T_BF16>(p, (hipStream_t)stream) : forward<T_F16>(p, (hipStream_t)stream);
   if (rc) return rc;
   OCTSAM_LAUNCH_CHECK("octsam_gated_fwd");
   return 0;
@@ -912,22 +1001,19 @@ extern "C" int octsam_gated_bwd(const void* dh, int64_t lddh, const void* gu, in
                    "gated_bwd: the workspace needs %lld bytes, 16-B aligned", (long long)b.total);
   const hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
-  const ActBwd a = {dh, gu, (const uint8_t*)gu_scale, dx || dw ? ws + b.dgu : nullptr, h, db ? (float*)(ws + b.part) : nullptr,
-                    lddh, ldgu, ld_gu_scale, 2 * (int64_t)F, ldh, M, b.slab, F, act};
-  if (xq && M > 0) {
-    if (int rc = octsam_dequant8(x, ldx, x_scale, ld_x_scale, M, D, ws + b.x16, type, D, stream)) return rc;
-    x = ws + b.x16;
+  ActBwd a = {};
+  a.dh = dh, a.lddh = lddh, a.gu = gu, a.ldgu = ldgu, a.gs = (const uint8_t*)gu_scale, a.ldgs = ld_gu_scale;
+  a.dgu = dx || dw ? ws + b.dgu : nullptr, a.lddgu = 2 * (int64_t)F;
+  a.h = h, a.ldh = ldh, a.part = db ? (float*)(ws + b.part) : nullptr;
+  a.M = M, a.F = F, a.act = act, a.slab = b.slab;
+  if (xq) {
+    a.x8 = x, a.ldx = ldx, a.xs = (const uint8_t*)x_scale, a.ldxs = ld_x_scale, a.D = D;
+    x = a.x16 = ws + b.x16;
     ldx = D;
   }
-  const int rc = type == T_BF16 ? run_bwd<T_BF16>(b, a, gu_type, x, ldx, w, ldw, M, D, F, dx, lddx, dw, dw_type, lddw, ws, s)
-                                : run_bwd<T_F16>(b, a, gu_type, x, ldx, w, ldw, M, D, F, dx, lddx, dw, dw_type, lddw, ws, s);
+  const int rc = type == T_BF16 ? run_bwd<T_BF16>(b, a, gu_type, x, ldx, w, ldw, M, D, F, dx, lddx, dw, dw_type, lddw, db, ws, s)
+                                : run_bwd<T_F16>(b, a, gu_type, x, ldx, w, ldw, M, D, F, dx, lddx, dw, dw_type, lddw, db, ws, s);
   if (rc) return rc;
   OCTSAM_LAUNCH_CHECK("octsam_gated_bwd");
-  if (!db) return 0;
-  if (M == 0) {
-    hipLaunchKernelGGL(gated_zero_kernel, dim3((unsigned)((2ll * F + 255) / 256)), dim3(256), 0, s, db, 2ll * F);
-    OCTSAM_LAUNCH_CHECK("octsam_gated_bwd");
-    return 0;
-  }
-  return octsam_splitk_reduce((const float*)(ws + b.part), db, 2 * (int64_t)F, b.slabs, 0.0f, stream);
+  return 0;
 }

@@ -11,9 +11,11 @@
 // lane j holding the columns 8 (j + T c) .. + 7 in registers between the statistics and the outputs, so every operand
 // is read once in 16-B (fp32: 2 x 16-B) pieces and four neighbouring lanes hold an 8-bit group. The backward keeps
 // dw's columns in registers over a workgroup's rows, adds its row groups through LDS and leaves one partial row per
-// workgroup (octsam_splitk_reduce adds them in fixed order: results do not vary from run to run). Widths that are no
-// multiple of 8, strides and addresses off 16 bytes and rows over 8192 columns take the kernels that go column by
-// column with a wave per row and read the row twice.
+// workgroup, which a second launch adds in fixed order (results do not vary from run to run). Lanes past the row's end
+// load its first columns and drop them, so that no branch stands between one load and the next. Widths that are no
+// multiple of 8 and strides and addresses off 16 bytes take the same kernels with single elements (W = 1: lane j holds
+// the columns j + T i, 32 lanes an 8-bit group). Rows over 8192 columns go column by column with a wave per row and are
+// read twice.
 #include "q8.h"
 #include "../../include/octsam.h"
 
@@ -32,6 +34,49 @@ struct NormFwd {
   float eps;
 };
 
+// a lane's elements of its row: NCH chunks of 8, element e of chunk c at column col_of(c, e). W = 8: 8 consecutive
+// columns, all inside the row or all outside; W = 1: every element by itself
+template <int T, int W>
+__device__ __forceinline__ int col_of(int lane, int c, int e) { return W == 8 ? 8 * (lane + T * c) + e : lane + T * (8 * c + e); }
+template <int TY, int T, int W>
+__device__ __forceinline__ void load_chunk(const void* p, long long at, int lane, int c, int D, float* v) {
+  if constexpr (W == 8) {
+    const int col = col_of<T, W>(lane, c, 0);
+    load8<TY>(p, at + (col < D ? col : 0), v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int col = col_of<T, W>(lane, c, e);
+      v[e] = load1<TY>(p, at + (col < D ? col : 0));
+    }
+  }
+}
+// zeros in the place of columns past the row's end (D = 0: all)
+template <int T, int W>
+__device__ __forceinline__ void cut_chunk(int lane, int c, int D, float* v) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = col_of<T, W>(lane, c, e) < D ? v[e] : 0.0f;
+}
+template <int TY, int T, int W>
+__device__ __forceinline__ void store_chunk(void* p, long long at, int lane, int c, int D, const float* v) {
+  if constexpr (W == 8) {
+    const int col = col_of<T, W>(lane, c, 0);
+    if (col < D) store8<TY>(p, at + col, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int col = col_of<T, W>(lane, c, e);
+      if (col < D) store1<TY>(p, at + col, v[e]);
+    }
+  }
+}
+template <int T, int W>
+__device__ __forceinline__ void store_chunk_by(int type, void* p, long long at, int lane, int c, int D, const float* v) {
+  if (type == T_BF16) store_chunk<T_BF16, T, W>(p, at, lane, c, D, v);
+  else if (type == T_F32) store_chunk<T_F32, T, W>(p, at, lane, c, D, v);
+  else store_chunk<T_F16, T, W>(p, at, lane, c, D, v);
+}
+
 template <int T>
 __device__ __forceinline__ float group_total(float v, float* red) {
 #pragma unroll
@@ -47,18 +92,13 @@ __device__ __forceinline__ float group_total(float v, float* red) {
   return v;
 }
 
-__device__ __forceinline__ void store8_by(int type, void* p, long long i, const float* v) {
-  if (type == T_BF16) store8<T_BF16>(p, i, v);
-  else if (type == T_F32) store8<T_F32>(p, i, v);
-  else store8<T_F16>(p, i, v);
-}
 __device__ __forceinline__ void store1_by(int type, void* p, long long i, float v) {
   if (type == T_BF16) store1<T_BF16>(p, i, v);
   else if (type == T_F32) store1<T_F32>(p, i, v);
   else store1<T_F16>(p, i, v);
 }
 
-template <int XT, int RT, int T, int NCH>
+template <int XT, int RT, int T, int NCH, int W>
 __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(NormFwd a) {
   constexpr int RPB = 256 / T;
   __shared__ float red[4];
@@ -66,28 +106,22 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(NormFwd a) {
   const float inv_d = 1.0f / (float)a.D;
   const long long last = (a.rows + RPB - 1) / RPB * RPB;  // (all lanes of a wave run every pass: they reduce together)
   for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / T; row < last; row += (long long)gridDim.x * RPB) {
-    const bool in = row < a.rows;
-    float v[NCH][8];
+    const int D = row < a.rows ? a.D : 0;  // (a row past the end has no columns; it loads the last row's)
+    const long long from = row < a.rows ? row : a.rows - 1;
+    float v[NCH][8], r[RT != T_NONE ? NCH : 1][8];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = 8 * (lane + T * c);
-      if (in && col < a.D) load8<XT>(a.x, row * a.ldx + col, v[c]);
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] = 0.0f;
+      load_chunk<XT, T, W>(a.x, from * a.ldx, lane, c, a.D, v[c]);
+      if constexpr (RT != T_NONE) load_chunk<RT, T, W>(a.r, from * a.ldr, lane, c, a.D, r[c]);
     }
-    if constexpr (RT != T_NONE) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const int col = 8 * (lane + T * c);
-        if (in && col < a.D) {
-          float t[8];
-          load8<RT>(a.r, row * a.ldr + col, t);
+    for (int c = 0; c < NCH; ++c) {
+      if constexpr (RT != T_NONE) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[c][e] += t[e];
-          if (a.s) store8<RT>(a.s, row * a.lds + col, v[c]);
-        }
+        for (int e = 0; e < 8; ++e) v[c][e] += r[c][e];
+        if (a.s) store_chunk<RT, T, W>(a.s, row * a.lds, lane, c, D, v[c]);
       }
+      cut_chunk<T, W>(lane, c, D, v[c]);
     }
     float ss = 0.0f;
 #pragma unroll
@@ -96,30 +130,42 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(NormFwd a) {
       for (int e = 0; e < 8; ++e) ss = fmaf(v[c][e], v[c][e], ss);
     ss = group_total<T>(ss, red);
     const float rstd = 1.0f / sqrtf(fmaf(ss, inv_d, a.eps));
-    if (in && lane == 0 && a.rstd) a.rstd[row] = rstd;
+    if (D && lane == 0 && a.rstd) a.rstd[row] = rstd;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = 8 * (lane + T * c);
-      const bool on = in && col < a.D;
-      float m = 0.0f;
-      if (on) {
-        float w[8];
-        load8<T_F32>(a.w, col, w);
+      float w[8];
+      load_chunk<T_F32, T, W>(a.w, 0, lane, c, a.D, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[c][e] = v[c][e] * rstd * w[e];
-          m = fmaxf(m, finite_abs(v[c][e]));
-        }
-        if (a.y) store8_by(a.y_type, a.y, row * a.ldy + col, v[c]);
-      }
+      for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * rstd * w[e];
+      cut_chunk<T, W>(lane, c, D, v[c]);
+      if (a.y) store_chunk_by<T, W>(a.y_type, a.y, row * a.ldy, lane, c, D, v[c]);
       if (a.q) {  // (uniform)
-        m = fmaxf(m, __shfl_xor(m, 1, 64));
-        m = fmaxf(m, __shfl_xor(m, 2, 64));
-        if (on) {
-          const int b = q8_scale(m);
-          const float inv = q8_inverse(b);
-          *(u32x2*)(a.q + row * a.ldq + col) = (u32x2){q8_pack4(v[c], inv), q8_pack4(v[c] + 4, inv)};
-          if ((lane & 3) == 0) a.sc[row * a.ldsc + (col >> 5)] = (uint8_t)b;
+        if constexpr (W == 8) {
+          float m = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[c][e]));
+          m = fmaxf(m, __shfl_xor(m, 1, 64));
+          m = fmaxf(m, __shfl_xor(m, 2, 64));
+          const int col = col_of<T, W>(lane, c, 0);
+          if (col < D) {
+            const int b = q8_scale(m);
+            const float inv = q8_inverse(b);
+            *(u32x2*)(a.q + row * a.ldq + col) = (u32x2){q8_pack4(v[c], inv), q8_pack4(v[c] + 4, inv)};
+            if ((lane & 3) == 0) a.sc[row * a.ldsc + (col >> 5)] = (uint8_t)b;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float m = finite_abs(v[c][e]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            const int col = col_of<T, W>(lane, c, e);
+            if (col < D) {
+              const int b = q8_scale(m);
+              a.q[row * a.ldq + col] = q8_pack1(v[c][e], q8_inverse(b));
+              if ((lane & 31) == 0) a.sc[row * a.ldsc + (col >> 5)] = (uint8_t)b;
+            }
+          }
         }
       }
     }
@@ -180,33 +226,33 @@ struct NormBwd {
 };
 
 template <int ST>
-__device__ __forceinline__ void load_s8(const NormBwd& a, long long row, int col, float* v) {
-  if constexpr (ST == T_Q8) {
-    const u32x2 q = *(const u32x2*)((const uint8_t*)a.s + row * a.lds + col);
-    const float k = q8_value(a.sc[row * a.ldsc + (col >> 5)]);
-    q8_unpack4(q[0], k, v);
-    q8_unpack4(q[1], k, v + 4);
-  } else {
-    load8<ST>(a.s, row * a.lds + col, v);
-  }
-}
-template <int ST>
 __device__ __forceinline__ float load_s1(const NormBwd& a, long long row, int col) {
   if constexpr (ST == T_Q8)
     return q8_unpack1(((const uint8_t*)a.s)[row * a.lds + col], q8_value(a.sc[row * a.ldsc + (col >> 5)]));
   else
     return load1<ST>(a.s, row * a.lds + col);
 }
-__device__ __forceinline__ void add8_by(int type, const void* p, long long i, float* v) {
-  float t[8];
-  if (type == T_BF16) load8<T_BF16>(p, i, t);
-  else if (type == T_F32) load8<T_F32>(p, i, t);
-  else load8<T_F16>(p, i, t);
+template <int ST, int T, int W>
+__device__ __forceinline__ void load_s_chunk(const NormBwd& a, long long row, int lane, int c, float* v) {
+  if constexpr (ST != T_Q8) {
+    load_chunk<ST, T, W>(a.s, row * a.lds, lane, c, a.D, v);
+  } else if constexpr (W == 8) {
+    int col = col_of<T, W>(lane, c, 0);
+    col = col < a.D ? col : 0;
+    const u32x2 q = *(const u32x2*)((const uint8_t*)a.s + row * a.lds + col);
+    const float k = q8_value(a.sc[row * a.ldsc + (col >> 5)]);
+    q8_unpack4(q[0], k, v);
+    q8_unpack4(q[1], k, v + 4);
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] += t[e];
+    for (int e = 0; e < 8; ++e) {
+      const int col = col_of<T, W>(lane, c, e);
+      v[e] = load_s1<ST>(a, row, col < a.D ? col : 0);
+    }
+  }
 }
 
-template <int DT, int ST, int T, int NCH>
+template <int DT, int ST, int T, int NCH, int W>
 __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(NormBwd a) {
   constexpr int RPB = 256 / T;
   __shared__ float red[4];
@@ -216,33 +262,42 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(NormBwd a) {
   float w[NCH][8], dw[NCH][8];
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
-    const int col = 8 * (lane + T * c);
-    if (col < a.D) load8<T_F32>(a.w, col, w[c]);
-    else
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[c][e] = 0.0f;
+    load_chunk<T_F32, T, W>(a.w, 0, lane, c, a.D, w[c]);
+    cut_chunk<T, W>(lane, c, a.D, w[c]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[c][e] = 0.0f;
   }
   const long long last = (a.rows + RPB - 1) / RPB * RPB;
   for (long long row = (long long)blockIdx.x * RPB + sub; row < last; row += (long long)gridDim.x * RPB) {
-    const bool in = row < a.rows;
-    const float rstd = in ? a.rstd[row] : 0.0f;
-    float g[NCH][8], n[NCH][8];
+    const int D = row < a.rows ? a.D : 0;  // (a row past the end has no columns; it loads the last row's)
+    const long long from = row < a.rows ? row : a.rows - 1;
+    const float rstd = a.rstd[from];
+    float g[NCH][8], n[NCH][8], o[NCH][8];
     float dot = 0.0f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = 8 * (lane + T * c);
-      if (in && col < a.D) {
-        load8<DT>(a.dy, row * a.lddy + col, g[c]);
-        load_s8<ST>(a, row, col, n[c]);
-      } else {
+      load_chunk<DT, T, W>(a.dy, from * a.lddy, lane, c, a.D, g[c]);
+      load_s_chunk<ST, T, W>(a, from, lane, c, n[c]);
+    }
+    if (!a.dres) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[c][e] = n[c][e] = 0.0f;
-      }
+      for (int c = 0; c < NCH; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[c][e] = 0.0f;
+    } else if (a.dx_type == T_BF16) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) load_chunk<T_BF16, T, W>(a.dres, from * a.lddres, lane, c, a.D, o[c]);
+    } else if (a.dx_type == T_F32) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) load_chunk<T_F32, T, W>(a.dres, from * a.lddres, lane, c, a.D, o[c]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) load_chunk<T_F16, T, W>(a.dres, from * a.lddres, lane, c, a.D, o[c]);
     }
 #pragma unroll
-    for (int c = 0; c < NCH; ++c)
+    for (int c = 0; c < NCH; ++c) {
+      cut_chunk<T, W>(lane, c, D, g[c]);
+      cut_chunk<T, W>(lane, c, D, n[c]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         n[c][e] *= rstd;
@@ -250,17 +305,13 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(NormBwd a) {
         g[c][e] *= w[c][e];
         dot = fmaf(g[c][e], n[c][e], dot);
       }
+    }
     dot = group_total<T>(dot, red) * inv_d;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = 8 * (lane + T * c);
-      if (in && col < a.D) {
-        float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = rstd * (g[c][e] - n[c][e] * dot);
-        if (a.dres) add8_by(a.dx_type, a.dres, row * a.lddres + col, o);
-        store8_by(a.dx_type, a.dx, row * a.lddx + col, o);
-      }
+      for (int e = 0; e < 8; ++e) o[c][e] += rstd * (g[c][e] - n[c][e] * dot);
+      store_chunk_by<T, W>(a.dx_type, a.dx, row * a.lddx, lane, c, D, o[c]);
     }
   }
   if constexpr (RPB > 1) {
@@ -280,10 +331,7 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(NormBwd a) {
   }
   if (sub == 0) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      const int col = 8 * (lane + T * c);
-      if (col < a.D) store8<T_F32>(a.part, (long long)blockIdx.x * a.D + col, dw[c]);
-    }
+    for (int c = 0; c < NCH; ++c) store_chunk<T_F32, T, W>(a.part, (long long)blockIdx.x * a.D, lane, c, a.D, dw[c]);
   }
 }
 
@@ -322,50 +370,60 @@ __global__ __launch_bounds__(256) void rmsnorm_dw_any_kernel(NormBwd a) {
     a.part[(long long)blockIdx.y * a.D + c] = fold[0][lane] + fold[1][lane] + fold[2][lane] + fold[3][lane];
 }
 
-__global__ void zero_kernel(float* p, long long n) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) p[i] = 0.0f;
+// dw from the workgroups' partial rows (none: zero)
+__global__ __launch_bounds__(256) void dw_sum_kernel(const float* part, int rows, int D, float* dw) {
+  column_sums(part, rows, D, blockIdx.x * 32, dw);
 }
 
 constexpr int MAX_BLOCKS = 1024;  // workgroups of the backward, i.e. partial rows of dw
 
 bool vec_ok(const void* p, long long ld, int bytes) { return !p || (ld % 8 == 0 && aligned(p, bytes)); }
 
-// T, NCH by width: the fewest registers that hold the row (a wave's lanes are split over rows up to 256 columns)
-#define BY_WIDTH(D, GO)             \
-  if ((D) <= 128) { GO(16, 1) }     \
-  else if ((D) <= 256) { GO(32, 1) }   \
-  else if ((D) <= 512) { GO(64, 1) }   \
-  else if ((D) <= 1024) { GO(64, 2) }  \
-  else if ((D) <= 1536) { GO(64, 3) }  \
-  else if ((D) <= 2048) { GO(64, 4) }  \
-  else if ((D) <= 4096) { GO(256, 2) } \
-  else { GO(256, 4) }
+// T, NCH, W by width: the fewest registers that hold the row (a wave's lanes are split over rows up to 256 columns;
+// single elements need the 32 lanes of an 8-bit group)
+#define BY_WIDTH(D, VEC, GO)                                      \
+  if (VEC) {                                                      \
+    if ((D) <= 128) { GO(16, 1, 8) }                              \
+    else if ((D) <= 256) { GO(32, 1, 8) }                         \
+    else if ((D) <= 512) { GO(64, 1, 8) }                         \
+    else if ((D) <= 1024) { GO(64, 2, 8) }                        \
+    else if ((D) <= 1536) { GO(64, 3, 8) }                        \
+    else if ((D) <= 2048) { GO(64, 4, 8) }                        \
+    else if ((D) <= 4096) { GO(256, 2, 8) }                       \
+    else { GO(256, 4, 8) }                                        \
+  } else {                                                        \
+    if ((D) <= 256) { GO(32, 1, 1) }                              \
+    else if ((D) <= 512) { GO(64, 1, 1) }                         \
+    else if ((D) <= 1024) { GO(64, 2, 1) }                        \
+    else if ((D) <= 2048) { GO(64, 4, 1) }                        \
+    else { GO(256, 4, 1) }                                        \
+  }
+constexpr int MAX_D = 8192;  // widest row that is held in registers
 
 template <int XT, int RT>
 void launch_fwd(const NormFwd& a, bool vec, hipStream_t s) {
-  if (!vec) {
+  if (a.D > MAX_D) {
     const long long nb = (a.rows + 3) / 4;
     hipLaunchKernelGGL((rmsnorm_fwd_any_kernel<XT, RT>), dim3((unsigned)(nb < 65536 ? nb : 65536)), dim3(256), 0, s, a);
     return;
   }
-#define GO(T, NCH)                                                                                               \
+#define GO(T, NCH, W)                                                                                            \
   const long long nb = (a.rows + 256 / T - 1) / (256 / T);                                                       \
-  hipLaunchKernelGGL((rmsnorm_fwd_kernel<XT, RT, T, NCH>), dim3((unsigned)(nb < 65536 ? nb : 65536)), dim3(256), 0, s, a);
-  BY_WIDTH(a.D, GO)
+  hipLaunchKernelGGL((rmsnorm_fwd_kernel<XT, RT, T, NCH, W>), dim3((unsigned)(nb < 65536 ? nb : 65536)), dim3(256), 0, s, a);
+  BY_WIDTH(a.D, vec, GO)
 #undef GO
 }
 
 template <int DT, int ST>
 void launch_bwd(const NormBwd& a, bool vec, int nb, hipStream_t s) {
-  if (!vec) {
+  if (a.D > MAX_D) {
     hipLaunchKernelGGL((rmsnorm_dw_any_kernel<DT, ST>), dim3((unsigned)((a.D + 63) / 64), (unsigned)nb), dim3(256), 0, s, a);
     const long long n = (a.rows + 3) / 4;
     hipLaunchKernelGGL((rmsnorm_bwd_any_kernel<DT, ST>), dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, s, a);
     return;
   }
-#define GO(T, NCH) hipLaunchKernelGGL((rmsnorm_bwd_kernel<DT, ST, T, NCH>), dim3((unsigned)nb), dim3(256), 0, s, a);
-  BY_WIDTH(a.D, GO)
+#define GO(T, NCH, W) hipLaunchKernelGGL((rmsnorm_bwd_kernel<DT, ST, T, NCH, W>), dim3((unsigned)nb), dim3(256), 0, s, a);
+  BY_WIDTH(a.D, vec, GO)
 #undef GO
 }
 
@@ -396,7 +454,7 @@ extern "C" int octsam_rmsnorm_fwd(const void* x, int32_t x_type, int64_t ldx, co
                    "rmsnorm_fwd: an operand is not aligned to its type");
   const NormFwd a = {x, r, w, sum_out, y, (uint8_t*)q, (uint8_t*)scale, rstd, ldx, ldr, ld_sum, ldy, ldq, ld_scale, rows, D,
                      y_type, eps};
-  const bool vec = D % 8 == 0 && D <= 8192 && vec_ok(x, ldx, 16) && vec_ok(r, ldr, 16) && vec_ok(sum_out, ld_sum, 16) &&
+  const bool vec = D % 8 == 0 && vec_ok(x, ldx, 16) && vec_ok(r, ldr, 16) && vec_ok(sum_out, ld_sum, 16) &&
                    vec_ok(y, ldy, 16) && vec_ok(q, ldq, 8) && aligned(w, 16);
   const hipStream_t s = (hipStream_t)stream;
 #define RUN(XT)                                              \
@@ -411,7 +469,8 @@ extern "C" int octsam_rmsnorm_fwd(const void* x, int32_t x_type, int64_t ldx, co
 
 extern "C" int64_t octsam_rmsnorm_bwd_workspace(int64_t rows, int32_t D) {
   if (rows < 0 || D <= 0) return 0;
-  return (int64_t)bwd_blocks(rows) * D * (int64_t)sizeof(float);
+  const int nb = bwd_blocks(rows);
+  return nb == 1 ? 0 : (int64_t)nb * D * (int64_t)sizeof(float);
 }
 
 extern "C" int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy, const void* s, int32_t s_type, int64_t lds,
@@ -423,7 +482,7 @@ extern "C" int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy,
   OCTSAM_CHECK_ARG(dw, "rmsnorm_bwd: null operand");
   const hipStream_t st = (hipStream_t)stream;
   if (rows == 0) {
-    hipLaunchKernelGGL(zero_kernel, dim3((unsigned)((D + 255) / 256)), dim3(256), 0, st, dw, (long long)D);
+    hipLaunchKernelGGL(dw_sum_kernel, dim3((unsigned)((D + 31) / 32)), dim3(256), 0, st, (const float*)nullptr, 0, D, dw);
     OCTSAM_LAUNCH_CHECK("octsam_rmsnorm_bwd");
     return 0;
   }
@@ -440,7 +499,7 @@ extern "C" int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy,
                    "rmsnorm_bwd: the workspace needs %lld bytes, 16-B aligned", (long long)octsam_rmsnorm_bwd_workspace(rows, D));
   const NormBwd a = {dy, s, (const uint8_t*)s_scale, rstd, w, dres, dx, nb == 1 ? dw : (float*)workspace,
                      lddy, lds, ld_scale, lddres, lddx, rows, D, dx_type};
-  const bool vec = D % 8 == 0 && D <= 8192 && vec_ok(dy, lddy, 16) && vec_ok(s, lds, s_type == T_Q8 ? 8 : 16) &&
+  const bool vec = D % 8 == 0 && vec_ok(dy, lddy, 16) && vec_ok(s, lds, s_type == T_Q8 ? 8 : 16) &&
                    vec_ok(dres, lddres, 16) && vec_ok(dx, lddx, 16) && aligned(w, 16) && aligned(a.part, 16);
 #define RUN(DT)                                                 \
   if (s_type == T_BF16) launch_bwd<DT, T_BF16>(a, vec, nb, st); \
@@ -449,6 +508,8 @@ extern "C" int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy,
   else launch_bwd<DT, T_Q8>(a, vec, nb, st);
   if (dy_type == T_BF16) { RUN(T_BF16) } else if (dy_type == T_F32) { RUN(T_F32) } else { RUN(T_F16) }
 #undef RUN
+  if (nb > 1)
+    hipLaunchKernelGGL(dw_sum_kernel, dim3((unsigned)((D + 31) / 32)), dim3(256), 0, st, (const float*)workspace, nb, D, dw);
   OCTSAM_LAUNCH_CHECK("octsam_rmsnorm_bwd");
-  return nb == 1 ? 0 : octsam_splitk_reduce((const float*)workspace, dw, D, nb, 0.0f, stream);
+  return 0;
 }

@@ -253,6 +253,8 @@ def _rows(t, what):
     shape = t.shape
     if len(shape) == 2:
         rows, cols = shape
+        if t.is_contiguous():
+            return rows, cols, cols
         ld, sc = t.stride()
         if sc != 1 and cols > 1:
             raise ValueError(f"{what}: columns must be contiguous")
@@ -291,26 +293,15 @@ def _q8_pair(pair, rows, cols, what):
     return q, _like(q, rows, cols, what), scale, _like(scale, rows, (cols + 31) // 32, what + " scales")
 
 
-def _device_of(*ts):
+def _device_of(first, *ts):
     """The one device that all given tensors are on."""
-    dev = None
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("octsam kernels take device tensors only")
     for t in ts:
-        if t is not None:
-            if not t.is_cuda:
-                raise ValueError("octsam kernels take device tensors only")
-            if dev is None:
-                dev = t.device
-            elif t.device != dev:
-                raise ValueError(f"octsam kernels take tensors of one device, got {dev} and {t.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"octsam kernels take device tensors only, all of one device: got {dev} and {t.device}")
     return dev
-
-
-def _call_on(dev, name, *args):
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args)
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args)
 
 
 def q8_empty(shape, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -329,7 +320,7 @@ def quant8(x: torch.Tensor, q8=None) -> tuple[torch.Tensor, torch.Tensor]:
     dev = _device_of(x, *q8)
     rows, cols, ldx = _rows(x, "x")
     q, ldq, scale, lds = _q8_pair(q8, rows, cols, "q8")
-    _call_on(dev, "octsam_quant8", ptr(x), _type(x, "x"), ldx, rows, cols, ptr(q), ldq, ptr(scale), lds)
+    _lib.call_on(dev, "octsam_quant8", ptr(x), _type(x, "x"), ldx, rows, cols, ptr(q), ldq, ptr(scale), lds)
     return q8
 
 
@@ -338,7 +329,7 @@ def dequant8(q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> torch.T
     dev = _device_of(q, scale, out)
     rows, cols, ldo = _rows(out, "out")
     q, ldq, scale, lds = _q8_pair((q, scale), rows, cols, "q")
-    _call_on(dev, "octsam_dequant8", ptr(q), ldq, ptr(scale), lds, rows, cols, ptr(out), _type(out, "out"), ldo)
+    _lib.call_on(dev, "octsam_dequant8", ptr(q), ldq, ptr(scale), lds, rows, cols, ptr(out), _type(out, "out"), ldo)
     return out
 
 
@@ -367,7 +358,7 @@ def rmsnorm_fwd(x: torch.Tensor, w: torch.Tensor, eps: float, out: torch.Tensor 
         q, ldq, scale, ldsc = _q8_pair(q8, rows, D, "q8")
     if rstd is not None:
         _vector(rstd, rows, "rstd")
-    _call_on(dev, "octsam_rmsnorm_fwd", ptr(x), xt, ldx, ptr(residual), rt, ldr, ptr(w), rows, D, float(eps), ptr(sum_out),
+    _lib.call_on(dev, "octsam_rmsnorm_fwd", ptr(x), xt, ldx, ptr(residual), rt, ldr, ptr(w), rows, D, float(eps), ptr(sum_out),
              lds, ptr(out), yt, ldy, ptr(q), ldq, ptr(scale), ldsc, ptr(rstd))
     return out
 
@@ -399,8 +390,8 @@ def rmsnorm_bwd(dy: torch.Tensor, s, rstd: torch.Tensor, w: torch.Tensor, dx: to
     else:
         _vector(dw, D, "dw")
     nbytes = _lib.load().octsam_rmsnorm_bwd_workspace(rows, D)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    _call_on(dev, "octsam_rmsnorm_bwd", ptr(dy), _type(dy, "dy"), lddy, ptr(sv), st, lds, ptr(sc), ldsc, ptr(rstd), ptr(w),
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    _lib.call_on(dev, "octsam_rmsnorm_bwd", ptr(dy), _type(dy, "dy"), lddy, ptr(sv), st, lds, ptr(sc), ldsc, ptr(rstd), ptr(w),
              rows, D, ptr(dres), lddres, ptr(dx), xt, lddx, ptr(dw), ptr(ws), nbytes)
     return dx, dw
 
@@ -446,7 +437,7 @@ def gated_fwd(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, act: int =
     st = ldsv = ldsc = 0
     if save is not None:
         sv, st, ldsv, sc, ldsc = _kept(save, ty, M, F, "save")
-    _call_on(dev, "octsam_gated_fwd", ptr(x), ldx, ptr(w), ldw, ptr(bias), M, D, F, act, ty, ptr(out), ldh, ptr(sv), st, ldsv,
+    _lib.call_on(dev, "octsam_gated_fwd", ptr(x), ldx, ptr(w), ldw, ptr(bias), M, D, F, act, ty, ptr(out), ldh, ptr(sv), st, ldsv,
              ptr(sc), ldsc)
     return out
 
@@ -487,7 +478,7 @@ def gated_bwd(dh: torch.Tensor, saved, x, w: torch.Tensor, *, act: int = _lib.AC
         _vector(db, 2 * F, "db")
     nbytes = _lib.load().octsam_gated_bwd_workspace(M, D, F, int(xt == _Q8))
     ws = torch.empty(max(nbytes, 16), device=dev, dtype=torch.uint8)
-    _call_on(dev, "octsam_gated_bwd", ptr(dh), lddh, ptr(sv), st, ldsv, ptr(sc), ldsc, ptr(xv), xt, ldx, ptr(xs), ldxs, ptr(w),
+    _lib.call_on(dev, "octsam_gated_bwd", ptr(dh), lddh, ptr(sv), st, ldsv, ptr(sc), ldsc, ptr(xv), xt, ldx, ptr(xs), ldxs, ptr(w),
              ldw, M, D, F, act, ty, ptr(h), ldh, ptr(dx), lddx, ptr(dw), wt, lddw, ptr(db), ptr(ws), nbytes)
 
 

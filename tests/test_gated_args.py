@@ -114,7 +114,7 @@ def test_wrapper_checks(monkeypatch):
 
     def never(*a):
         raise AssertionError("launched")
-    monkeypatch.setattr(kernels, "_call_on", never)
+    monkeypatch.setattr(_lib, "call_on", never)
     bf = torch.bfloat16
     x, w, h = torch.zeros(4, 64, dtype=bf), torch.zeros(32, 64, dtype=bf), torch.zeros(4, 16, dtype=bf)
     wn, q = torch.ones(64), kernels.q8_empty((4, 64), "cpu")
