@@ -15,6 +15,7 @@
 // Operands with k contiguous and operands stored [k][x] (W in dx, both in dW) use the same loop: the second kind is
 // read from LDS with the transposing 64-bit read. Global loads run three K-steps ahead in registers.
 #include "q8.h"
+#include <math.h>
 #include <stdlib.h>
 #include "../../include/octsam.h"
 
@@ -511,15 +512,14 @@ __device__ __forceinline__ void place(int id, int tiles_m, int tiles_n, int& tm,
 // the `rest` others K is cut into `splits` parts, all tiles at the same places; of the rest * splits parts, in the order
 // part-major, the first `wgs` are a workgroup's first job each, so that what runs together on an XCD walks the same K
 // over neighbouring tiles and shares its panels in L2 (cut end to end into equal runs instead, every workgroup walked a
-// K of its own: dw of 16384 x 1280 x 3416 353 us, against 230). What is left, `over` tiles' last parts, is laid end to
-// end and cut into wgs equal runs, the second jobs, each in at most two tiles. All jobs leave fp32 partial tiles (slot w,
-// then wgs + 2 w and wgs + 2 w + 1), and gated_fix_kernel adds a tile's in order. wgs = 0: every tile is whole.
+// K of its own: dw of 16384 x 1280 x 3416 353 us, against 230). What is left, `over` tiles' last parts, is cut into
+// `runs` each, the second jobs of the first over * runs workgroups: more runs end sooner but each leaves a partial tile
+// of 256 KiB. All jobs leave fp32 partial tiles (slot w, then wgs + w), and gated_fix_kernel adds a tile's in order.
+// wgs = 0: every tile is whole.
 struct Share {
-  int tiles_m, tiles_n, steps, whole, rest, splits, wgs, over;
+  int tiles_m, tiles_n, steps, whole, rest, splits, wgs, over, runs;
 };
 __device__ __host__ __forceinline__ int part_start(const Share& s, int j) { return (int)((long long)j * s.steps / s.splits); }
-__device__ __host__ __forceinline__ int last_part(const Share& s) { return s.steps - part_start(s, s.splits - 1); }
-__device__ __host__ __forceinline__ int run_start(const Share& s, int w) { return (int)((long long)w * s.over * last_part(s) / s.wgs); }
 
 template <int TY, int MODE>
 __global__ __launch_bounds__(512, 2) void gated_big_kernel(GatedP p, Share sh, float* part) {
@@ -547,19 +547,12 @@ __global__ __launch_bounds__(512, 2) void gated_big_kernel(GatedP p, Share sh, f
       q.M = q.N = 256;
       store256<TY, MODE>(q, 0, 0, acc, wave, lane);
     };
-    const int end = run_start(sh, w + 1), len = last_part(sh), k_last = part_start(sh, sh.splits - 1);
-    int u = run_start(sh, w);
-    const int j0 = w / sh.rest;
-    int t = w - j0 * sh.rest, kb = part_start(sh, j0), n = part_start(sh, j0 + 1) - kb, slot = w;
-    for (int k = 0;; ++k) {
-      job(t, kb, n, slot);
-      if (u >= end) break;
-      const int l = u / len, in = u - l * len;
-      t = sh.rest - sh.over + l;
-      kb = k_last + in;
-      n = end - u < len - in ? end - u : len - in;
-      slot = sh.wgs + 2 * w + k;
-      u += n;
+    const int j = w / sh.rest, kb = part_start(sh, j);
+    job(w - j * sh.rest, kb, part_start(sh, j + 1) - kb, w);
+    if (w < sh.over * sh.runs) {
+      const int l = w / sh.runs, i = w - l * sh.runs, k0 = part_start(sh, sh.splits - 1), len = sh.steps - k0;
+      const int from = (int)((long long)i * len / sh.runs), to = (int)((long long)(i + 1) * len / sh.runs);
+      job(sh.rest - sh.over + l, k0 + from, to - from, sh.wgs + w);
     }
   }
 }
@@ -574,33 +567,30 @@ __global__ __launch_bounds__(256) void gated_fix_kernel(GatedP p, Share sh, cons
   const int n = tn * 256 + c;
   if (m >= p.M || n >= p.N) return;
   float v[8] = {};
-  auto add = [&](int slot) {
-    float x[8];
-    load8<T_F32>(part, (long long)slot * 65536 + r * 256 + c, x);
+  // `count` partials, `step` slots apart, four in flight
+  auto add = [&](int slot, int step, int count) {
+    const float* at = part + (long long)slot * 65536 + r * 256 + c;
+    const long long by = (long long)step * 65536;
+    int j = 0;
+    for (; j + 4 <= count; j += 4) {
+      float x[4][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += x[e];
-  };
-  const int l = t - (sh.rest - sh.over);  // >= 0: the last part was shared out over runs
-  const int mains = l < 0 ? sh.splits : sh.splits - 1;
-  int j = 0;
-  for (; j + 4 <= mains; j += 4) {  // (four partials in flight)
-    float x[4][8];
+      for (int i = 0; i < 4; ++i) load8<T_F32>(at, (j + i) * by, x[i]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load8<T_F32>(part, (long long)((j + i) * sh.rest + t) * 65536 + r * 256 + c, x[i]);
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += x[i][e];
-  }
-  for (; j < mains; ++j) add(j * sh.rest + t);
-  if (l >= 0) {
-    const long long len = last_part(sh), a = l * len, b = a + len, units = sh.over * len;
-    const int w0 = (int)(((a + 1) * sh.wgs - 1) / units), w1 = (int)((b * sh.wgs - 1) / units);  // runs of units a and b - 1
-    for (int w = w0; w <= w1; ++w) {
-      const int u = run_start(sh, w);
-      if (u < run_start(sh, w + 1)) add(sh.wgs + 2 * w + (u < a));
+        for (int e = 0; e < 8; ++e) v[e] += x[i][e];
     }
-  }
+    for (; j < count; ++j) {
+      float x[8];
+      load8<T_F32>(at, j * by, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += x[e];
+    }
+  };
+  const int l = t - (sh.rest - sh.over);  // >= 0: the last part was a second job
+  add(t, sh.rest, l < 0 ? sh.splits : sh.splits - 1);
+  if (l >= 0) add(sh.wgs + l * sh.runs, 1, sh.runs);
   if (p.c_type == T_F32) store8<T_F32>(p.C, m * p.ldc + n, v);
   else store8<TY>(p.C, m * p.ldc + n, v);
 }
@@ -765,7 +755,8 @@ JoinJob join_job(TileJob& j, void* ws) {
   return f;
 }
 
-// shares a product of 256 x 256 tiles out; sharing costs about 10 K-steps (16 us: second jobs and the adding)
+// Shares a product of 256 x 256 tiles out where that is shorter, in K-steps of a workgroup (1.75 us with the chip full): a
+// partial tile's way to memory and back takes 0.07 of them (256 KiB twice at 4 TB/s), second jobs and launches 4
 Share share_out(Mode mode, long long M, long long N, long long K) {
   Share s = {};
   const int per = mode == GATED ? 128 : 256;
@@ -776,23 +767,29 @@ Share share_out(Mode mode, long long M, long long N, long long K) {
   s.rest = (int)(tiles % 256);
   s.whole = (int)tiles;
   s.splits = 1;
-  if (mode == GATED || s.rest == 0 || s.steps < 8) return s;
-  int splits = (256 + s.rest - 1) / s.rest, over = 0;
+  if (mode == GATED || s.rest == 0) return s;
+  int splits = (255 + s.rest) / s.rest;
   if (splits > s.steps / 4) splits = s.steps / 4;
-  int wgs = s.rest * splits;
+  if (splits < 2) return s;
+  int wgs = s.rest * splits, over = 0, runs = 0;
+  const double part = (double)s.steps / splits, partial = 0.07;
+  double shared = part + 4;
   if (wgs > 256) {
     over = wgs - 256;
     wgs = 256;
+    runs = (int)sqrt(part / (partial * over));  // part / runs + partial * over * runs at its least
+    const int most = 256 / over < (int)part / 2 ? 256 / over : (int)part / 2;
+    runs = runs > most ? most : runs;
+    runs = runs < 1 ? 1 : runs;
+    shared += part / runs;
   }
+  shared += partial * (wgs + over * runs);
+  if (shared > s.steps) return s;
   s.splits = splits;
-  const double shared = (double)s.steps / splits + (double)over * last_part(s) / wgs + 10;
-  if (splits < 2 || shared > s.steps) {
-    s.splits = 1;
-    return s;
-  }
   s.whole = (int)(tiles - s.rest);
   s.wgs = wgs;
   s.over = over;
+  s.runs = runs;
   return s;
 }
 
@@ -832,7 +829,7 @@ int64_t tiles_of(int64_t M, int64_t N) { return ((M + 63) / 64) * ((N + 63) / 64
 int64_t partial_bytes(Mode mode, int64_t M, int64_t N, int64_t K, int64_t tiles) {
   if (M <= 0 || N <= 0) return 0;
   const Share sh = share_out(mode, M, N, K);
-  const int64_t big = (int64_t)sh.wgs * (sh.over ? 3 : 1) * 65536 * 4;
+  const int64_t big = (int64_t)(sh.wgs + sh.over * sh.runs) * 65536 * 4;
   GatedP p = {};
   p.M = (int)M;
   p.N = (int)N;
@@ -844,7 +841,7 @@ int64_t partial_bytes(Mode mode, int64_t M, int64_t N, int64_t K, int64_t tiles)
 
 // rows per workgroup of the element-wise backward (grid y: at most 32768 workgroups)
 int64_t slab_of(int64_t M) {
-  const int64_t least = (M + 32767) / 32768, want = M <= 64 ? 8 : M <= 2048 ? 32 : 64;
+  const int64_t least = (M + 32767) / 32768, want = M <= 2048 ? 8 : M <= 8192 ? 32 : 64;
   return least > want ? (least + 7) / 8 * 8 : want;
 }
 
