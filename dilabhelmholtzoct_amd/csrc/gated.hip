@@ -9,14 +9,12 @@
 // step, 2^-9 relative in bf16, against results that are rounded to the same step); db is summed from the unrounded
 // fp32 values.
 //
-// Tile: 64 x 64 x 64, four waves of 16 rows x 64 columns of 16x16x32 MFMAs with swapped operands (a lane holds 4
-// consecutive columns of a row; one permlane16_swap makes 8). In the forward the 64 columns are 32 gate rows and the 32
-// up rows of the same features, so a lane has g and u of the same 8 features and four lanes hold an 8-bit group.
-// Operands with k contiguous and operands stored [k][x] (W in dx, both in dW) use the same loop: the second kind is
-// read from LDS with the transposing 64-bit read. Global loads run three K-steps ahead in registers.
+// All tiles run 16x16x32 MFMAs with swapped operands (a lane holds 4 consecutive columns of a row; one permlane16_swap
+// makes 8). In the forward a wave's 64 columns are 32 gate rows and the 32 up rows of the same features, so a lane has g
+// and u of the same 8 features and four lanes hold an 8-bit group. Operands with k contiguous and operands stored
+// [k][x] (W in dx, both in dW) use the same loops: the second kind is read from LDS with the transposing 64-bit read.
 #include "q8.h"
 #include <math.h>
-#include <stdlib.h>
 #include "../../include/octsam.h"
 
 namespace {
@@ -165,126 +163,158 @@ __device__ __forceinline__ void plain_store(const GatedP& p, long long m, int n,
   else store8<TY>(p.C, at, v);
 }
 
-// ------------------------------------------------------------------------------------------------------- 64 x 64 tile
-// LDS images [64 rows][128 B]; 16-B chunk c of row r sits at c ^ swizzle. Rows of k (KC): (r >> 1) & 7, the 16 rows of
-// a fragment read land on 16 slots. [k][x] (KM): the four rows q of a 16-lane group and the group pair (r bit 3) land
-// on 8 slot pairs of two rows.
+// ------------------------------------------------------------------------------------- 64 x 64 and 128 x 128 tiles
+// LDS images. Rows of k (KC): [T rows][128 B], 16-B chunk c of row r at c ^ (r >> 1) & 7: the 16 rows of a fragment read
+// land on 16 slots. [k][x] (KM): [64 rows][2 T B]; a transposing read takes four rows q and two groups of rows (r bit 3)
+// at once: T = 64, two rows to 256 bytes, the swizzle gives them 4 slot pairs; T = 128, 8 slot pairs.
 __device__ __forceinline__ int kc_at(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
-__device__ __forceinline__ int km_at(int r, int c) { return r * 128 + ((c ^ ((r & 2) | ((r >> 1) & 4))) << 4); }
+template <int T>
+__device__ __forceinline__ int km_at(int r, int c) {
+  if constexpr (T == 64) return r * 128 + ((c ^ ((r & 2) | ((r >> 1) & 4))) << 4);
+  else return r * 256 + ((c ^ (((r & 3) << 2) | ((r >> 2) & 2))) << 4);
+}
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-template <int TY, bool KM>
-__device__ __forceinline__ typename Elem<TY>::v8 frag64(const char* img, int x0, int kb, int lane) {
+// the 16 x 32 fragment of rows (columns of a KM image) x0 .. x0 + 15, k half kh
+template <int TY, bool KM, int T>
+__device__ __forceinline__ typename Elem<TY>::v8 fragment(const char* img, int x0, int kh, int lane) {
   typedef typename Elem<TY>::v8 v8;
   if constexpr (!KM) {
-    return *(const v8*)(img + kc_at(x0 + (lane & 15), kb * 4 + (lane >> 4)));
+    return *(const v8*)(img + kc_at(x0 + (lane & 15), kh * 4 + (lane >> 4)));
   } else {
     const int g = lane >> 4, i = lane & 15, q = i >> 2, pp = i & 3;
-    const char* at = img + km_at(kb * 32 + 8 * g + q, (x0 >> 3) + (pp >> 1)) + 8 * (pp & 1);
+    const char* at = img + km_at<T>(kh * 32 + 8 * g + q, (x0 >> 3) + (pp >> 1)) + 8 * (pp & 1);
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * 128));  // (+4 leaves the swizzle)
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * 2 * T));  // (+4 leaves the swizzle)
     const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(v8, v);
   }
 }
 
-typedef char TileLds[2][2][64 * 128];  // [stage][operand]
+// T x T tiles by four waves: T = 64, 16 rows x 64 columns each; T = 128, 64 x 64 each (half the LDS reads an MFMA, where
+// there are tiles enough). In the forward the columns are gate and up rows in turns of 32, T / 2 features.
+template <int T>
+struct TileLds {
+  char stage[2][2][T * 128];  // [stage][operand]
+};
 
 // tile `tile` (column tiles first) of K split `split`
-template <int TY, int MODE>
-__device__ __forceinline__ void tile64(const GatedP& p, int tiles_n, int tile, int split, TileLds& smem) {
+template <int TY, int MODE, int T>
+__device__ __forceinline__ void tile(const GatedP& p, int tiles_n, int tile, int split, TileLds<T>& smem) {
   typedef typename Elem<TY>::v8 v8;
   constexpr bool AKM = MODE == TN, BKM = MODE != GATED;
-  constexpr int AHEAD = 3;
+  constexpr int AHEAD = T == 64 ? 3 : 2, NP = T / 32, MB = T == 64 ? 1 : 4, XC = T / 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tm = tile / tiles_n, tn = tile - tm * tiles_n;
-  const long long row0 = (long long)tm * 64;
-  const int col0 = tn * (MODE == GATED ? 32 : 64);
+  const long long row0 = (long long)tm * T;
+  const int col0 = tn * (MODE == GATED ? T / 2 : T);
   const long long k0 = (long long)split * p.kper;
   const int kn = (int)(p.K - k0 < p.kper ? p.K - k0 : p.kper);  // (< 1: no steps, the tile is zero)
   const int steps = kn > 0 ? (kn + 63) / 64 : 0;
 
-  // this thread's two 16-B pieces of each operand's stage: image row rr (and rr + 32), chunk cc
-  const int rr = tid >> 3, cc = tid & 7;
-  const char *pa[2], *pb[2];
-  bool oa[2], ob[2];
+  // this thread's NP 16-B pieces of each operand's stage: image row r (k for KM), chunk c; at: its place in the image
+  const char *pa[NP], *pb[NP];
+  int ka[NP], kb[NP], la[NP], lb[NP];  // k of the piece (past K: never, where its row is none of the operand's)
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = rr + 32 * i;
+  for (int i = 0; i < NP; ++i) {
+    const int id = tid + 256 * i;
     if constexpr (AKM) {
-      oa[i] = row0 + cc * 8 < p.M;
-      pa[i] = (const char*)p.A + ((k0 + r) * p.lda + row0 + cc * 8) * 2;
+      const int r = id / XC, c = id % XC;
+      ka[i] = row0 + c * 8 < p.M ? r : 1 << 30;
+      la[i] = km_at<T>(r, c);
+      pa[i] = (const char*)p.A + ((k0 + r) * p.lda + row0 + c * 8) * 2;
     } else {
-      oa[i] = row0 + r < p.M;
-      pa[i] = (const char*)p.A + ((row0 + r) * p.lda + k0 + cc * 8) * 2;
+      const int r = id >> 3, c = id & 7;
+      ka[i] = row0 + r < p.M ? c * 8 : 1 << 30;
+      la[i] = kc_at(r, c);
+      pa[i] = (const char*)p.A + ((row0 + r) * p.lda + k0 + c * 8) * 2;
     }
     if constexpr (BKM) {
-      ob[i] = col0 + cc * 8 < p.N;
-      pb[i] = (const char*)p.B + ((k0 + r) * p.ldb + col0 + cc * 8) * 2;
+      const int r = id / XC, c = id % XC;
+      kb[i] = col0 + c * 8 < p.N ? r : 1 << 30;
+      lb[i] = km_at<T>(r, c);
+      pb[i] = (const char*)p.B + ((k0 + r) * p.ldb + col0 + c * 8) * 2;
     } else {
-      ob[i] = col0 + rr < p.N;  // image rows 0-31: gate features, 32-63: the same features' up rows
-      pb[i] = (const char*)p.B + (((long long)i * p.N + col0 + rr) * p.ldb + k0 + cc * 8) * 2;
+      const int r = id >> 3, c = id & 7, f = col0 + (r >> 6) * 32 + (r & 31);  // row r: gate (r bit 5 = 0) or up row of f
+      kb[i] = f < p.N ? c * 8 : 1 << 30;
+      lb[i] = kc_at(r, c);
+      pb[i] = (const char*)p.B + (((long long)((r >> 5) & 1) * p.N + f) * p.ldb + k0 + c * 8) * 2;
     }
   }
   const long long sa = AKM ? p.lda * 128 : 128, sb = BKM ? p.ldb * 128 : 128;
-  u32x4 ra[AHEAD][2], rb[AHEAD][2];
-  auto fetch = [&](int t, u32x4 (&a)[2], u32x4 (&b)[2]) {
+  u32x4 ra[AHEAD][NP], rb[AHEAD][NP];
+  auto fetch = [&](int t, u32x4 (&a)[NP], u32x4 (&b)[NP]) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int ka = t * 64 + (AKM ? rr + 32 * i : cc * 8), kb = t * 64 + (BKM ? rr + 32 * i : cc * 8);
-      a[i] = oa[i] && ka < kn ? *(const u32x4*)(pa[i] + t * sa) : (u32x4)0u;
-      b[i] = ob[i] && kb < kn ? *(const u32x4*)(pb[i] + t * sb) : (u32x4)0u;
+    for (int i = 0; i < NP; ++i) {
+      a[i] = t * 64 + ka[i] < kn ? *(const u32x4*)(pa[i] + t * sa) : (u32x4)0u;
+      b[i] = t * 64 + kb[i] < kn ? *(const u32x4*)(pb[i] + t * sb) : (u32x4)0u;
     }
   };
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j)
     if (j < steps) fetch(j, ra[j], rb[j]);
-  f32x4 acc[4] = {(f32x4)0.0f, (f32x4)0.0f, (f32x4)0.0f, (f32x4)0.0f};
+  f32x4 acc[MB][4];
+#pragma unroll
+  for (int mi = 0; mi < MB; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4)0.0f;
+  const int wrow = T == 64 ? wave * 16 : (wave >> 1) * 64, wcol = T == 64 ? 0 : (wave & 1) * 64;
   for (int t0 = 0; t0 < steps; t0 += AHEAD) {
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int t = t0 + j;
       if (t < steps) {
-        char *ia = smem[t & 1][0], *ib = smem[t & 1][1];
+        char *ia = smem.stage[t & 1][0], *ib = smem.stage[t & 1][1];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          *(u32x4*)(ia + (AKM ? km_at(rr + 32 * i, cc) : kc_at(rr + 32 * i, cc))) = ra[j][i];
-          *(u32x4*)(ib + (BKM ? km_at(rr + 32 * i, cc) : kc_at(rr + 32 * i, cc))) = rb[j][i];
+        for (int i = 0; i < NP; ++i) {
+          *(u32x4*)(ia + la[i]) = ra[j][i];
+          *(u32x4*)(ib + lb[i]) = rb[j][i];
         }
         if (t + AHEAD < steps) fetch(t + AHEAD, ra[j], rb[j]);
         // one barrier a step: whoever writes this buffer again has passed the next step's barrier, and so have all
         // its readers of this step
         __syncthreads();
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const v8 af = frag64<TY, AKM>(ia, wave * 16, kb, lane);
+        for (int kh = 0; kh < 2; ++kh) {
+          v8 af[MB];
 #pragma unroll
-          for (int ni = 0; ni < 4; ++ni) acc[ni] = mma<TY>(frag64<TY, BKM>(ib, ni * 16, kb, lane), af, acc[ni]);
+          for (int mi = 0; mi < MB; ++mi) af[mi] = fragment<TY, AKM, T>(ia, wrow + mi * 16, kh, lane);
+#pragma unroll
+          for (int ni = 0; ni < 4; ++ni) {
+            const v8 bf = fragment<TY, BKM, T>(ib, wcol + ni * 16, kh, lane);
+#pragma unroll
+            for (int mi = 0; mi < MB; ++mi) acc[mi][ni] = mma<TY>(bf, af[mi], acc[mi][ni]);
+          }
         }
       }
     }
   }
   const int q = lane >> 4, cofs = 16 * (q & 1) + 8 * (q >> 1);
-  const long long m = row0 + wave * 16 + (lane & 15);
-  float v0[8], v1[8];
-  row8(acc[0], acc[1], v0);
-  row8(acc[2], acc[3], v1);
-  if constexpr (MODE == GATED) {
-    gated_store<TY>(p, m, col0 + cofs, load_bias(p, col0 + cofs), v0, v1);
-  } else {
-    plain_store<TY>(p, m, col0 + cofs, split, v0);
-    plain_store<TY>(p, m, col0 + 32 + cofs, split, v1);
+  Bias8 b;
+  if constexpr (MODE == GATED) b = load_bias(p, col0 + wcol / 2 + cofs);
+#pragma unroll
+  for (int mi = 0; mi < MB; ++mi) {
+    const long long m = row0 + wrow + mi * 16 + (lane & 15);
+    float v0[8], v1[8];
+    row8(acc[mi][0], acc[mi][1], v0);
+    row8(acc[mi][2], acc[mi][3], v1);
+    if constexpr (MODE == GATED) {
+      gated_store<TY>(p, m, col0 + wcol / 2 + cofs, b, v0, v1);
+    } else {
+      plain_store<TY>(p, m, col0 + wcol + cofs, split, v0);
+      plain_store<TY>(p, m, col0 + wcol + 32 + cofs, split, v1);
+    }
   }
 }
 
-template <int TY>
+template <int TY, int T>
 __global__ __launch_bounds__(256) void gated_tile_kernel(GatedP p, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) TileLds smem;
-  tile64<TY, GATED>(p, tiles_n, blockIdx.x, 0, smem);
+  __shared__ __attribute__((aligned(16))) TileLds<T> smem;
+  tile<TY, GATED, T>(p, tiles_n, blockIdx.x, 0, smem);
 }
 
 // both products of the backward in one launch: dx's tiles (each K split of all tiles in turn), then dw's
@@ -292,15 +322,15 @@ struct TileJob {
   GatedP p;
   int tiles, tiles_n, splits;
 };
-template <int TY>
+template <int TY, int T>
 __global__ __launch_bounds__(256) void gated_pair_kernel(TileJob x, TileJob w) {
-  __shared__ __attribute__((aligned(16))) TileLds smem;
+  __shared__ __attribute__((aligned(16))) TileLds<T> smem;
   int b = blockIdx.x;
   if (b < x.tiles * x.splits) {
-    tile64<TY, NN>(x.p, x.tiles_n, b % x.tiles, b / x.tiles, smem);
+    tile<TY, NN, T>(x.p, x.tiles_n, b % x.tiles, b / x.tiles, smem);
   } else {
     b -= x.tiles * x.splits;
-    tile64<TY, TN>(w.p, w.tiles_n, b % w.tiles, b / w.tiles, smem);
+    tile<TY, TN, T>(w.p, w.tiles_n, b % w.tiles, b / w.tiles, smem);
   }
 }
 
@@ -778,17 +808,32 @@ __global__ __launch_bounds__(256) void gated_act_bwd_kernel(ActBwd a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
-// A product on 64 x 64 tiles: K splits so that `tiles` (of all products of the launch) give the chip's 256 CUs three
-// workgroups each, at least four K-steps a split
-TileJob tile_job(const GatedP& p, long long tiles) {
+// The backward's two products. On 256 x 256 tiles, a launch each, from 12000 K-steps of both together (47 for each CU);
+// else on T x T tiles in one launch, `per` K-steps a workgroup, so that both run out at the same time and the chip has
+// about 512 (T = 128) or 1024 workgroups, at least 4 steps each. Counted from the sizes alone, whichever outputs are
+// asked for: alone and together they have the same bits. Measured (bf16, the whole backward, us; 256 / 128 / 64):
+// 16384 x 1024 x 2736 469 / 630 / -, 8192 x 768 x 2048 (12288 steps) 220 / 237 / -, 4096 x 1024 x 2736 (11136)
+// 177 / 183 / -, 4096 x 768 x 2048 160 / 101 / 134, 1024 x 768 x 2048 71 / 40 / 47, 128 x 1024 x 2736 43 / 27 / 24.6
+struct TilePlan {
+  int T, per;  // T = 256: per is for strides that the 256 x 256 kernel does not reach, on 128 x 128 tiles
+};
+int64_t tiles_of(int64_t M, int64_t N, int T) { return ((M + T - 1) / T) * ((N + T - 1) / T); }
+TilePlan tile_plan(int64_t M, int64_t D, int64_t F) {
+  auto units = [&](int T) { return tiles_of(M, D, T) * ((2 * F + 63) / 64) + tiles_of(2 * F, D, T) * ((M + 63) / 64); };
+  TilePlan t;
+  t.T = units(256) >= 12000 ? 256 : units(128) >= 2500 ? 128 : 64;
+  const int64_t slots = t.T == 64 ? 1024 : 512, per = (units(t.T == 64 ? 64 : 128) + slots - 1) / slots;
+  t.per = (int)(per < 4 ? 4 : per);
+  return t;
+}
+TileJob tile_job(const GatedP& p, const TilePlan& t) {
   TileJob j = {};
   j.p = p;
-  j.tiles_n = (p.N + 63) / 64;
-  j.tiles = (int)(((long long)p.M + 63) / 64 * j.tiles_n);
-  const int steps = (p.K + 63) / 64;
-  long long s = tiles > 0 ? (767 + tiles) / tiles : 1;
-  if (s > steps / 4) s = steps / 4;
-  j.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  const int T = t.T == 64 ? 64 : 128;
+  j.tiles_n = (p.N + T - 1) / T;
+  j.tiles = (int)tiles_of(p.M, p.N, T);
+  const int steps = (p.K + 63) / 64, s = (steps + t.per / 2) / t.per;
+  j.splits = s < 1 ? 1 : s > 64 ? 64 : s;
   j.p.kper = (steps + j.splits - 1) / j.splits * 64;
   return j;
 }
@@ -858,13 +903,8 @@ int product_big(const GatedP& p, const Share& sh, void* ws, hipStream_t s) {
     hipLaunchKernelGGL((gated_fix_kernel<TY>), dim3(32, (unsigned)sh.rest), dim3(256), 0, s, p, sh, (const float*)ws);
   return 0;
 }
-int big_from() {  // TEMP tuning
-  static const int v = getenv("GATED_BIG") ? atoi(getenv("GATED_BIG")) : 64;
-  return v;
-}
 // operand strides up to which the 256 x 256 kernel's 32-bit offsets reach
 bool near(int64_t ld) { return ld < (1 << 21); }
-bool use_big(const Share& s) { return (long long)s.tiles_m * s.tiles_n >= big_from() && s.steps > 0; }
 
 template <int TY>
 int forward(const GatedP& p, hipStream_t s) {
@@ -872,30 +912,33 @@ int forward(const GatedP& p, hipStream_t s) {
     hipLaunchKernelGGL((gated_few_kernel<TY>), dim3((unsigned)((p.N + 31) / 32)), dim3(64 * FEW_WAVES), 0, s, p);
     return 0;
   }
+  // The tile: 256 x 256 once its tiles fill more than half of the 256 CUs, 128 x 128 once its own fill most of them (two
+  // fit a CU), else 64 x 64. Measured (bf16, us; 256 / 128 / 64): 2048 x 1024 x 2736 31 / 40 / 51, 2048 x 768 x 2048
+  // (128 tiles) 23.0 / 21.0 / 29, 512 x 1280 x 3416 (54, 216) 30 / 22 / 29, 512 x 768 x 2048 (16, 128) 21 / 13.8 / 10.5
   const Share sh = share_out(GATED, p.M, p.N, p.K);
-  if (use_big(sh) && near(p.lda) && near(p.ldb)) return product_big<TY, GATED>(p, sh, nullptr, s);
-  const int tiles_n = (p.N + 31) / 32;
-  const long long tiles = ((long long)p.M + 63) / 64 * tiles_n;
-  OCTSAM_CHECK_ARG(tiles < (1ll << 31), "gated_fwd: too many tiles");
+  if (sh.whole >= 150 && near(p.lda) && near(p.ldb)) return product_big<TY, GATED>(p, sh, nullptr, s);
   GatedP q = p;
   q.kper = (p.K + 63) / 64 * 64;
-  hipLaunchKernelGGL((gated_tile_kernel<TY>), dim3((unsigned)tiles), dim3(256), 0, s, q, tiles_n);
+  const int64_t large = ((int64_t)p.M + 127) / 128 * (((int64_t)p.N + 63) / 64), small = ((int64_t)p.M + 63) / 64 * (((int64_t)p.N + 31) / 32);
+  OCTSAM_CHECK_ARG(small < (1ll << 31), "gated_fwd: too many tiles");
+  if (large >= 192)
+    hipLaunchKernelGGL((gated_tile_kernel<TY, 128>), dim3((unsigned)large), dim3(256), 0, s, q, (p.N + 63) / 64);
+  else
+    hipLaunchKernelGGL((gated_tile_kernel<TY, 64>), dim3((unsigned)small), dim3(256), 0, s, q, (p.N + 31) / 32);
   return 0;
 }
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
-int64_t tiles_of(int64_t M, int64_t N) { return ((M + 63) / 64) * ((N + 63) / 64); }
-// bytes of fp32 partials of a product: on 256 x 256 tiles, or (as strides far apart can ask for) on 64 x 64 tiles, of
-// which both products have `tiles`
-int64_t partial_bytes(Mode mode, int64_t M, int64_t N, int64_t K, int64_t tiles) {
+// bytes of fp32 partials of a product
+int64_t partial_bytes(Mode mode, int64_t M, int64_t N, int64_t K, const TilePlan& t) {
   if (M <= 0 || N <= 0) return 0;
   const Share sh = share_out(mode, M, N, K);
-  const int64_t big = (int64_t)(sh.wgs + sh.over * sh.runs) * 65536 * 4;
+  const int64_t big = t.T == 256 ? (int64_t)(sh.wgs + sh.over * sh.runs) * 65536 * 4 : 0;
   GatedP p = {};
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
-  const int splits = tile_job(p, tiles).splits;
+  const int splits = tile_job(p, t).splits;
   const int64_t small = splits > 1 ? splits * M * N * 4 : 0;
   return round16(big > small ? big : small);
 }
@@ -908,6 +951,7 @@ int64_t slab_of(int64_t M) {
 
 struct BwdPlan {
   int64_t dgu, x16, part, join_x, join_w, total;
+  TilePlan tiles;
   int64_t slab;
   int slabs;
 };
@@ -923,10 +967,10 @@ BwdPlan bwd_plan(int64_t M, int64_t D, int64_t F, bool x_q8) {
   b.part = at;
   at += round16((int64_t)b.slabs * 2 * F * 4);
   b.join_x = at;
-  const int64_t tiles = tiles_of(M, D) + tiles_of(2 * F, D);
-  at += partial_bytes(NN, M, D, 2 * F, tiles);
+  b.tiles = tile_plan(M, D, F);
+  at += partial_bytes(NN, M, D, 2 * F, b.tiles);
   b.join_w = at;
-  at += partial_bytes(TN, 2 * F, D, M, tiles);
+  at += partial_bytes(TN, 2 * F, D, M, b.tiles);
   b.total = at;
   return b;
 }
@@ -950,7 +994,7 @@ int run_bwd(const BwdPlan& b, const ActBwd& act, int gu_type, const void* x, int
   px.B = w, px.ldb = ldw, px.C = dx, px.ldc = lddx, px.c_type = TY, px.M = (int)M, px.K = 2 * F;
   pw.B = x, pw.ldb = ldx, pw.C = dw, pw.ldc = lddw, pw.c_type = dw_type, pw.M = 2 * F, pw.K = (int)M;
   const Share shx = share_out(NN, M, D, 2 * F), shw = share_out(TN, 2 * F, D, M);
-  const bool big_x = use_big(shx) && near(px.lda) && near(ldw), big_w = use_big(shw) && near(pw.lda) && near(ldx);
+  const bool big = b.tiles.T == 256 && near(px.lda), big_x = big && near(ldw), big_w = big && M > 0 && near(ldx);
   if (dx && M > 0 && big_x)
     if (int rc = product_big<TY, NN>(px, shx, ws + b.join_x, s)) return rc;
   if (dw && big_w)
@@ -959,12 +1003,13 @@ int run_bwd(const BwdPlan& b, const ActBwd& act, int gu_type, const void* x, int
   TileJob jx = {}, jw = {};
   JoinJob fx = {}, fw = {};
   if (tile_x || tile_w) {
-    const int64_t tiles = tiles_of(M, D) + tiles_of(2 * F, D);  // (whichever are asked for: the same bits)
-    OCTSAM_CHECK_ARG(tiles < (1 << 24), "gated_bwd: too many tiles");
-    if (tile_x) jx = tile_job(px, tiles), fx = join_job(jx, ws + b.join_x);
-    if (tile_w) jw = tile_job(pw, tiles), fw = join_job(jw, ws + b.join_w);
+    const int T = b.tiles.T == 64 ? 64 : 128;
+    OCTSAM_CHECK_ARG(tiles_of(M, D, T) + tiles_of(2 * F, D, T) < (1 << 24), "gated_bwd: too many tiles");
+    if (tile_x) jx = tile_job(px, b.tiles), fx = join_job(jx, ws + b.join_x);
+    if (tile_w) jw = tile_job(pw, b.tiles), fw = join_job(jw, ws + b.join_w);
     const int blocks = jx.tiles * jx.splits + jw.tiles * jw.splits;
-    hipLaunchKernelGGL((gated_pair_kernel<TY>), dim3((unsigned)blocks), dim3(256), 0, s, jx, jw);
+    if (T == 64) hipLaunchKernelGGL((gated_pair_kernel<TY, 64>), dim3((unsigned)blocks), dim3(256), 0, s, jx, jw);
+    else hipLaunchKernelGGL((gated_pair_kernel<TY, 128>), dim3((unsigned)blocks), dim3(256), 0, s, jx, jw);
   }
   DbJob d = {};
   if (db) {

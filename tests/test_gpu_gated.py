@@ -268,7 +268,12 @@ def code(name):
 
 GATED_SHAPES = [(1, 8, 8), (1, 256, 688), (2, 72, 40), (7, 264, 96), (16, 1280, 344), (17, 64, 32), (33, 320, 360), (64, 128, 64),
                 (65, 136, 72), (130, 512, 200), (257, 200, 264), (1029, 256, 688), (300, 768, 1032), (768, 72, 1288),
-                (2100, 328, 520)]
+                (2100, 328, 520),
+                # 128 x 128 tiles in the forward; 256 x 256
+                (520, 136, 3000), (2500, 72, 2056)]
+# the backward on 128 x 128 tiles; on 256 x 256: K cut over idle workgroups with second jobs (dw), a rest of 4 tiles behind
+# 256 whole ones (dx) and parts that come out even (dw)
+GATED_LARGE = [(1100, 520, 1032), (16400, 520, 1032), (16400, 1024, 1024)]
 
 
 @pytest.mark.parametrize("M,D,F", GATED_SHAPES)
@@ -336,7 +341,7 @@ def check_bwd(got, want, dh, gu, x, w, dtype, M, F):
         close(got["db"], want["db"], a.sum(0) * (M + 32) * U32 + slack.sum(0) + 1e-30)
 
 
-@pytest.mark.parametrize("M,D,F", GATED_SHAPES + [(0, 64, 40)])
+@pytest.mark.parametrize("M,D,F", GATED_SHAPES + GATED_LARGE + [(0, 64, 40)])
 @pytest.mark.parametrize("dtype,act,kept,x8,dwt", [(BF, "silu", "8", True, BF), (BF, "gelu", "16", False, F32),
                                                    (F16, "gelu", "8", True, F16), (F16, "silu", "16", False, F16),
                                                    (BF, "relu", "16", True, BF), (BF, "none", "8", False, BF)])
