@@ -84,30 +84,27 @@ __device__ __forceinline__ void row8(f32x4 a, f32x4 b, float* v) {
   }
 }
 
-// the largest of v over the four lanes (16 apart) that hold an 8-bit group
+// the largest of v over the four lanes (16 apart) that hold an 8-bit group: both results of a swap of v with itself hold
+// one half's values in both halves
 __device__ __forceinline__ float group_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  const uint32_t a = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const uint32_t b = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1])));
+  const auto t = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)t[0]), __builtin_bit_cast(float, (uint32_t)t[1]));
 }
-// amax ignores NaN; only where it is infinite are the finite values searched again
 __device__ __forceinline__ void keep8_q(const GatedP& p, long long m, int half, int f, bool ok, const float* v) {
-  float a = 0.0f;
+  float a = 0.0f, w[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e]));
-  a = group_max(ok ? a : 0.0f);
-  const bool inf = !is_finite(a);
-  if (__any(inf)) {
-    float b = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) b = fmaxf(b, finite_abs(v[e]));
-    b = group_max(ok ? b : 0.0f);
-    if (inf) a = b;
+  for (int e = 0; e < 8; ++e) {
+    w[e] = q8_clean(v[e]);
+    a = fmaxf(a, fabsf(w[e]));
   }
+  a = group_max(ok ? a : 0.0f);
   if (ok) {
     const int b = q8_scale(a);
     const float inv = q8_inverse(b);
-    *(u32x2*)((uint8_t*)p.save + m * p.ldsave + (long long)half * p.N + f) =
-        inf ? (u32x2){q8_pack4(v, inv), q8_pack4(v + 4, inv)} : (u32x2){q8_pack4_plain(v, inv), q8_pack4_plain(v + 4, inv)};
+    *(u32x2*)((uint8_t*)p.save + m * p.ldsave + (long long)half * p.N + f) = (u32x2){q8_pack4(w, inv), q8_pack4(w + 4, inv)};
     if ((f & 31) == 0) p.scale[m * p.ldscale + half * ((p.N + 31) / 32) + (f >> 5)] = (uint8_t)b;
   }
 }

@@ -32,27 +32,17 @@ __device__ __forceinline__ float q8_value(int b) {  // 2^(b - 127), b in [0, 255
   const uint32_t u = b == 0 ? 0x00400000u : b == 255 ? 0x7fc00000u : (uint32_t)b << 23;
   return __builtin_bit_cast(float, u);
 }
-__device__ __forceinline__ bool is_finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) != 0x7f800000u; }
-__device__ __forceinline__ float finite_abs(float x) { return is_finite(x) ? fabsf(x) : 0.0f; }
-// x * inv for the conversion: the product's magnitude is at most 448, or NaN
-__device__ __forceinline__ float q8_ready(float x, float inv) {
-  return is_finite(x) ? x * inv : __builtin_bit_cast(float, 0x7fc00000u);
-}
+// x, or NaN where it is not finite (inf * 0): what the functions below take. Maxima ignore NaN, products and the
+// conversion keep it
+__device__ __forceinline__ float q8_clean(float x) { return fmaf(x, 0.0f, x); }
 __device__ __forceinline__ uint32_t q8_pack4(const float* x, float inv) {
-  int r = 0;
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(q8_ready(x[0], inv), q8_ready(x[1], inv), r, false);
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(q8_ready(x[2], inv), q8_ready(x[3], inv), r, true);
-  return (uint32_t)r;
-}
-// the same for values known to be finite or NaN (a NaN's product is NaN)
-__device__ __forceinline__ uint32_t q8_pack4_plain(const float* x, float inv) {
   int r = 0;
   r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, r, false);
   r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, r, true);
   return (uint32_t)r;
 }
 __device__ __forceinline__ uint8_t q8_pack1(float x, float inv) {
-  return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(q8_ready(x, inv), 0.0f, 0, false) & 0xff);
+  return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(x * inv, 0.0f, 0, false) & 0xff);
 }
 __device__ __forceinline__ void q8_unpack4(uint32_t q, float s, float* x) {
   const f32x2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);

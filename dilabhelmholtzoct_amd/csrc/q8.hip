@@ -25,7 +25,10 @@ __global__ __launch_bounds__(256) void quant8_vec_kernel(const void* __restrict_
     if (on) {
       load8<TY>(x, r * ldx + c, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
+      for (int e = 0; e < 8; ++e) {
+        v[e] = q8_clean(v[e]);
+        m = fmaxf(m, fabsf(v[e]));
+      }
     }
     m = fmaxf(m, __shfl_xor(m, 1, 64));
     m = fmaxf(m, __shfl_xor(m, 2, 64));
@@ -49,8 +52,8 @@ __global__ __launch_bounds__(256) void quant8_any_kernel(const void* __restrict_
     const long long r = i / ngr;
     const int g = (int)(i - r * ngr), c = g * 32 + lane;
     const bool on = i < total && c < cols;
-    const float v = on ? load1<TY>(x, r * ldx + c) : 0.0f;
-    float m = finite_abs(v);
+    const float v = on ? q8_clean(load1<TY>(x, r * ldx + c)) : 0.0f;
+    float m = fmaxf(0.0f, fabsf(v));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     if (on) {

@@ -143,7 +143,10 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(NormFwd a) {
         if constexpr (W == 8) {
           float m = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[c][e]));
+          for (int e = 0; e < 8; ++e) {
+            v[c][e] = q8_clean(v[c][e]);
+            m = fmaxf(m, fabsf(v[c][e]));
+          }
           m = fmaxf(m, __shfl_xor(m, 1, 64));
           m = fmaxf(m, __shfl_xor(m, 2, 64));
           const int col = col_of<T, W>(lane, c, 0);
@@ -156,13 +159,14 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(NormFwd a) {
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            float m = finite_abs(v[c][e]);
+            const float y = q8_clean(v[c][e]);
+            float m = fmaxf(0.0f, fabsf(y));
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
             const int col = col_of<T, W>(lane, c, e);
             if (col < D) {
               const int b = q8_scale(m);
-              a.q[row * a.ldq + col] = q8_pack1(v[c][e], q8_inverse(b));
+              a.q[row * a.ldq + col] = q8_pack1(y, q8_inverse(b));
               if ((lane & 31) == 0) a.sc[row * a.ldsc + (col >> 5)] = (uint8_t)b;
             }
           }
@@ -201,7 +205,8 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_any_kernel(NormFwd a) {
         if (a.y) store1_by(a.y_type, a.y, row * a.ldy + c, y);
       }
       if (a.q) {
-        float m = finite_abs(y);
+        y = q8_clean(y);
+        float m = fmaxf(0.0f, fabsf(y));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
         if (on) {

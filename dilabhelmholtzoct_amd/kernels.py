@@ -251,29 +251,26 @@ def _type(t, what):
 def _rows(t, what):
     """(rows, columns, row stride) of t seen as rows of its last dimension."""
     shape = t.shape
-    if len(shape) == 2:
-        rows, cols = shape
-        if t.is_contiguous():
-            return rows, cols, cols
-        ld, sc = t.stride()
-        if sc != 1 and cols > 1:
-            raise ValueError(f"{what}: columns must be contiguous")
-        if rows <= 1:
-            ld = cols
-        elif ld < cols:
-            raise ValueError(f"{what}: rows overlap (row stride {ld}, width {cols})")
-        return rows, cols, ld
-    if not shape or not t.is_contiguous():
+    if t.is_contiguous() and shape:
+        cols = shape[-1]
+        return (t.numel() // cols if cols else 0), cols, cols
+    if len(shape) != 2:
         raise ValueError(f"{what}: [rows, columns] with any row stride, or contiguous [..., columns]")
-    cols = shape[-1]
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    return rows, cols, cols
+    rows, cols = shape
+    ld, sc = t.stride()
+    if sc != 1 and cols > 1:
+        raise ValueError(f"{what}: columns must be contiguous")
+    if rows <= 1:
+        ld = cols
+    elif ld < cols:
+        raise ValueError(f"{what}: rows overlap (row stride {ld}, width {cols})")
+    return rows, cols, ld
 
 
 def _like(t, rows, cols, what):
     """Row stride of t, which must be [rows, cols]."""
+    if t.is_contiguous() and t.numel() == rows * cols and t.dim() and t.shape[-1] == cols:
+        return cols
     r, c, ld = _rows(t, what)
     if r != rows or c != cols:
         raise ValueError(f"{what} is {tuple(t.shape)}: {rows} rows of {cols} are expected")
