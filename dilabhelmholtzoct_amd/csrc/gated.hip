@@ -331,20 +331,8 @@ __global__ __launch_bounds__(256) void gated_pair_kernel(TileJob x, TileJob w) {
   }
 }
 
-// ----------------------------------------------------------------------------------------------------- 256 x 256 tile
-// Large products: 256 x 256 x 64 tiles (GATED: 128 features, gate and up rows in turns of 32), eight waves as 2 (rows)
-// x 4 (columns) with 128 x 64 each, operands by LDS-DMA through buffer descriptors (what lies past an operand's end
-// reads as zero), two stages of 64 KiB. A K-step of a wave is two segments between barriers: L reads its 24 fragments
-// and issues its share of the DMA, C runs its 64 MFMAs; the two wave rows run one segment apart, so that each SIMD has
-// one wave in its MFMAs while its other wave loads. A's rows 0-127 are read by wave row 0 alone (segment 2t), 128-255
-// by wave row 1 (2t + 1), B by both, and a region is refilled once its last reader has passed a barrier:
-//   wave row 0 in L(t): B(t + 1), landed at the end of its C(t)
-//   wave row 1 in L(t): A-hi(t + 1), landed at the end of its C(t); A-lo(t + 2), landed at the end of its L(t + 1)
-//   before the loop:    stage 0 and A-lo(1)
-// LDS images: rows of k as above; [k][x] operands as two halves of 128 columns, [64][256 B], chunk c of row r at
-// c ^ 2 ((r & 3) << 1 | (r >> 3) & 1): a transposing read's 32 lanes (rows q of 4, and 8 + q) cover 16 chunk slots, and
-// a fragment's address is one xor of a lane constant with the column block, plus constants.
-constexpr int STAGE = 65536, OUT_OF_RANGE = (int)0x80000000;
+// ----------------------------------------------------------------------------------------------- for the large tiles
+constexpr int OUT_OF_RANGE = (int)0x80000000;
 
 __device__ __forceinline__ void hard_barrier() {
   asm volatile("" ::: "memory");
@@ -358,6 +346,156 @@ __device__ __forceinline__ void wait_loads() {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void* base, long long bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)(bytes > 0 ? bytes : 0), 0x00020000);
 }
+
+// tiles go to the XCDs (workgroup id mod 8) in contiguous runs, and within a run eight row tiles take turns over the
+// column tiles, so that what is in flight on an XCD shares row and column panels in its L2
+__device__ __forceinline__ int tile_of(int bid, int nwg) {
+  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, loc = bid >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + loc;
+}
+__device__ __forceinline__ void place(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int per = 8 * tiles_n, g = id / per, in = id - g * per;
+  const int h = tiles_m - g * 8 < 8 ? tiles_m - g * 8 : 8;
+  tn = in / h;
+  tm = g * 8 + (in - tn * h);
+}
+
+// ------------------------------------------------------------------------ the forward: two workgroups to a CU
+// 128 rows x 128 features (256 columns) x 64 tiles, four waves of 128 x 64. LDS holds one stage of A (16 KiB) and two of B
+// (64): 80 KiB, so two workgroups share a CU and each SIMD has a wave of either. A K-step is: wait for the stage; all 24
+// fragments into registers; barrier; A's next stage and B's next but one on their way; 64 MFMAs. K is short here (D) and
+// the epilogue long (activation, product, 8-bit groups: about 25 vector operations per element of h): while one workgroup
+// is in its epilogue, its first loads, a wait or its fragment reads, the other has the matrix cores.
+// 16384 x 1024 x 2736 bf16: 161 us (1140 TFLOP/s), with the 8-bit save 181; the 256 x 256 tiles below, one workgroup to a
+// CU, took 174 and 193 (for the backward's longer K they are ahead: dx 152 us against 187, with two thirds of the reads).
+// The fragment reads are assembly with their wait in the same block: as ordinary loads they would wait for all DMA in
+// flight.
+constexpr int DUO_B = 16384, DUO_LDS = 81920;
+
+// fragments of 16-row blocks 2048 bytes apart, k half by k half (a0, a1), from rows of k
+template <typename V>
+__device__ __forceinline__ void read_rows(V (&f)[8][2], uint32_t a0, uint32_t a1) {
+  asm volatile(
+      "ds_read_b128 %0, %16\n\tds_read_b128 %1, %17\n\tds_read_b128 %2, %16 offset:2048\n\tds_read_b128 %3, %17 offset:2048\n\t"
+      "ds_read_b128 %4, %16 offset:4096\n\tds_read_b128 %5, %17 offset:4096\n\t"
+      "ds_read_b128 %6, %16 offset:6144\n\tds_read_b128 %7, %17 offset:6144\n\t"
+      "ds_read_b128 %8, %16 offset:8192\n\tds_read_b128 %9, %17 offset:8192\n\t"
+      "ds_read_b128 %10, %16 offset:10240\n\tds_read_b128 %11, %17 offset:10240\n\t"
+      "ds_read_b128 %12, %16 offset:12288\n\tds_read_b128 %13, %17 offset:12288\n\t"
+      "ds_read_b128 %14, %16 offset:14336\n\tds_read_b128 %15, %17 offset:14336\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1]), "=&v"(f[2][0]), "=&v"(f[2][1]), "=&v"(f[3][0]),
+        "=&v"(f[3][1]), "=&v"(f[4][0]), "=&v"(f[4][1]), "=&v"(f[5][0]), "=&v"(f[5][1]), "=&v"(f[6][0]), "=&v"(f[6][1]),
+        "=&v"(f[7][0]), "=&v"(f[7][1])
+      : "v"(a0), "v"(a1)
+      : "memory");
+}
+template <typename V>
+__device__ __forceinline__ void read_rows(V (&f)[4][2], uint32_t a0, uint32_t a1) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %8 offset:2048\n\tds_read_b128 %3, %9 offset:2048\n\t"
+      "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\t"
+      "ds_read_b128 %6, %8 offset:6144\n\tds_read_b128 %7, %9 offset:6144\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1]), "=&v"(f[2][0]), "=&v"(f[2][1]), "=&v"(f[3][0]),
+        "=&v"(f[3][1])
+      : "v"(a0), "v"(a1)
+      : "memory");
+}
+template <int TY>
+__device__ __forceinline__ void duo_tile(const GatedP& p, int tiles_m, int tiles_n, char* lds) {
+  typedef typename Elem<TY>::v8 v8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tm, tn;
+  place(tile_of(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
+  const long long row0 = (long long)tm * 128;
+  const int col0 = tn * 128, n = (p.K + 63) / 64;
+  const long long lda2 = p.lda * 2, ldb2 = p.ldb * 2;
+  // a lane's part of a 1 KiB DMA piece (8 rows of 128 B), by the piece's parity: its chunk's k and its offset
+  int kc[2], va[2], vb[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = e * 8 + (lane >> 3);
+    kc[e] = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+    va[e] = (int)(r * lda2) + kc[e] * 2;
+    vb[e] = (int)(r * ldb2) + kc[e] * 2;
+  }
+  const int nf = p.N - col0 < 128 ? p.N - col0 : 128;
+  const __amdgpu_buffer_rsrc_t ra = range((const char*)p.A + row0 * lda2, (p.M - row0 < 128 ? p.M - row0 : 128) * lda2);
+  const __amdgpu_buffer_rsrc_t rg = range((const char*)p.B + (long long)col0 * ldb2, nf * ldb2);
+  const __amdgpu_buffer_rsrc_t ru = range((const char*)p.B + ((long long)p.N + col0) * ldb2, nf * ldb2);
+  // (only the last K-step of a K that is no multiple of 64 has chunks past K)
+  auto cut = [&](int v, int e, int t) { return t * 64 + 64 <= p.K || t * 64 + kc[e] < p.K ? v : OUT_OF_RANGE; };
+  auto load_a = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(lds + (wave * 4 + i) * 1024), 16, cut(va[i & 1], i & 1, t),
+                                               (int)((wave * 32 + (i & ~1) * 8) * lda2) + t * 128, 0, 0);
+  };
+  auto load_b = [&](int t) {  // image rows 64 wave + (0-31: gate features 32 wave .., 32-63: the same features' up rows)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < 4 ? rg : ru, (lds_ptr_t)(lds + DUO_B + (t & 1) * 32768 + (wave * 8 + i) * 1024), 16,
+                                               cut(vb[i & 1], i & 1, t), (int)((wave * 32 + (i & 2) * 8) * ldb2) + t * 128, 0, 0);
+  };
+  f32x4 acc[8][4];
+#pragma unroll
+  for (int mi = 0; mi < 8; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4)0.0f;
+  const int fr = lane & 15;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds, row_at = fr * 128 + (((lane >> 4) ^ ((fr >> 1) & 7)) << 4);
+  load_b(0);
+  load_a(0);
+  if (n > 1) load_b(1);
+  for (int t = 0; t < n; ++t) {
+    if (t + 1 < n) wait_loads<8>();  // (loads land in order: all but B(t + 1))
+    else wait_loads<0>();
+    hard_barrier();
+    v8 af[8][2], bf[4][2];
+    const uint32_t ib = lds0 + DUO_B + (t & 1) * 32768 + wave * 8192 + row_at;
+    read_rows(bf, ib, ib ^ 64);
+    read_rows(af, lds0 + row_at, lds0 + (row_at ^ 64));
+    hard_barrier();  // (every wave has its fragments: A's stage and this one of B may be written)
+    if (t + 1 < n) load_a(t + 1);
+    if (t + 2 < n) load_b(t + 2);
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int mi = 0; mi < 8; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = mma<TY>(bf[ni][kh], af[mi][kh], acc[mi][ni]);
+  }
+  const int q = lane >> 4, f = col0 + wave * 32 + 16 * (q & 1) + 8 * (q >> 1);
+  const Bias8 b = load_bias(p, f);
+#pragma unroll
+  for (int mi = 0; mi < 8; ++mi) {
+    float g[8], u[8];
+    row8(acc[mi][0], acc[mi][1], g);
+    row8(acc[mi][2], acc[mi][3], u);
+    gated_store<TY>(p, row0 + mi * 16 + (lane & 15), f, b, g, u);
+  }
+}
+template <int TY>
+__global__ __launch_bounds__(256, 2) void gated_duo_kernel(GatedP p, int tiles_m, int tiles_n) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  duo_tile<TY>(p, tiles_m, tiles_n, lds);
+}
+
+// ----------------------------------------------------------------------------------------------------- 256 x 256 tile
+// The backward's large products: 256 x 256 x 64 tiles, eight waves as 2 (rows) x 4 (columns) with 128 x 64 each, operands
+// by LDS-DMA through buffer descriptors (what lies past an operand's end reads as zero), two stages of 64 KiB. A K-step of a wave is two segments between barriers: L reads its 24 fragments
+// and issues its share of the DMA, C runs its 64 MFMAs; the two wave rows run one segment apart, so that each SIMD has
+// one wave in its MFMAs while its other wave loads. A's rows 0-127 are read by wave row 0 alone (segment 2t), 128-255
+// by wave row 1 (2t + 1), B by both, and a region is refilled once its last reader has passed a barrier:
+//   wave row 0 in L(t): B(t + 1), landed at the end of its C(t)
+//   wave row 1 in L(t): A-hi(t + 1), landed at the end of its C(t); A-lo(t + 2), landed at the end of its L(t + 1)
+//   before the loop:    stage 0 and A-lo(1)
+// LDS images: rows of k as above; [k][x] operands as two halves of 128 columns, [64][256 B], chunk c of row r at
+// c ^ 2 ((r & 3) << 1 | (r >> 3) & 1): a transposing read's 32 lanes (rows q of 4, and 8 + q) cover 16 chunk slots, and
+// a fragment's address is one xor of a lane constant with the column block, plus constants.
+// 16384 x 5472 x 1024 (dx) 152 us, 1210 TFLOP/s, MFMAs busy 60 % at the 2.0 GHz that the chip holds. What bounds it is the
+// way of every K-step's new lines into the XCD's L2: the DMA alone, nothing computed, takes 147 us (out of L2 it could
+// run at half that), fragment reads alone 67. Three stages of B did not shorten it.
+constexpr int STAGE = 65536;
 
 template <int TY, bool KM>
 __device__ __forceinline__ typename Elem<TY>::v8 frag256(const char* img, int x0, int kb, int lane) {
@@ -380,7 +518,7 @@ template <int TY, int MODE>
 __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col0, int kb, int n, f32x4 (&acc)[8][4], char* lds,
                                         int wave, int lane) {
   typedef typename Elem<TY>::v8 v8;
-  constexpr bool AKM = MODE == TN, BKM = MODE != GATED;
+  constexpr bool AKM = MODE == TN;  // (B is [k][x] in both)
   const int wr = wave >> 2, wc = wave & 3;
   const long long lda2 = p.lda * 2, ldb2 = p.ldb * 2;
   const char *A = (const char*)p.A, *B = (const char*)p.B;
@@ -395,11 +533,8 @@ __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col
 #pragma unroll
   for (int e = 0; e < 2; ++e) va[e] = lane_part(AKM, e, lda2);
 #pragma unroll
-  for (int e = 0; e < 2; ++e) vb[e] = lane_part(BKM, e, ldb2);
+  for (int e = 0; e < 2; ++e) vb[e] = lane_part(true, e, ldb2);
   const __amdgpu_buffer_rsrc_t ra = range(A + row0 * lda2, (p.M - row0 < 256 ? p.M - row0 : 256) * lda2);
-  const int nf = p.N - col0 < 128 ? p.N - col0 : 128;
-  const __amdgpu_buffer_rsrc_t rg = range(B + (long long)col0 * ldb2, nf * ldb2);
-  const __amdgpu_buffer_rsrc_t ru = range(B + ((long long)p.N + col0) * ldb2, nf * ldb2);
   // 16-B chunk of a row of k that lies past K (only in the last K-step of a K that is no multiple of 64)
   auto cut = [&](int v, int e, int t) {
     const int r = e * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
@@ -419,14 +554,8 @@ __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col
   };
   auto dma_b = [&](int j, int t) {  // piece j (of 32) of B, stage t
     const lds_ptr_t dst = (lds_ptr_t)(lds + (t & 1) * STAGE + 32768 + j * 1024);
-    if constexpr (BKM) {
-      const int h = j >> 4, jj = j & 15;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(km_range(B, ldb2, col0 + h * 128, p.N, t), dst, 16, vb[(jj >> 1) & 1], (int)(4 * jj * ldb2), 0, 0);
-    } else {
-      const int jj = j & 7;  // image rows 64 w + (0-31: gate features 32 w .., 32-63: the same features' up rows)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(jj < 4 ? rg : ru, dst, 16, cut(vb[j & 1], j & 1, t),
-                                               (int)(((j >> 3) * 32 + (jj & 2) * 8) * ldb2) + (kb + t) * 128, 0, 0);
-    }
+    const int h = j >> 4, jj = j & 15;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(km_range(B, ldb2, col0 + h * 128, p.N, t), dst, 16, vb[(jj >> 1) & 1], (int)(4 * jj * ldb2), 0, 0);
   };
 #pragma unroll
   for (int mi = 0; mi < 8; ++mi)
@@ -453,10 +582,8 @@ __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
 #pragma unroll
-      for (int ni = 0; ni < 4; ++ni) {
-        if constexpr (BKM) bf[ni][kh] = frag256<TY, true>(cur + 32768 + (wc >> 1) * 16384, (wc & 1) * 64 + ni * 16, kh, lane);
-        else bf[ni][kh] = frag256<TY, false>(cur + 32768, wc * 64 + ni * 16, kh, lane);
-      }
+      for (int ni = 0; ni < 4; ++ni)
+        bf[ni][kh] = frag256<TY, true>(cur + 32768 + (wc >> 1) * 16384, (wc & 1) * 64 + ni * 16, kh, lane);
 #pragma unroll
       for (int mi = 0; mi < 8; ++mi) {
         if constexpr (AKM) af[mi][kh] = frag256<TY, true>(cur + wr * 16384, mi * 16, kh, lane);
@@ -502,37 +629,18 @@ __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col
   }
 }
 
-template <int TY, int MODE>
+template <int TY>
 __device__ __forceinline__ void store256(const GatedP& p, long long row0, int col0, f32x4 (&acc)[8][4], int wave, int lane) {
   const int wr = wave >> 2, wc = wave & 3, q = lane >> 4, cofs = 16 * (q & 1) + 8 * (q >> 1);
-  Bias8 b;
-  if constexpr (MODE == GATED) b = load_bias(p, col0 + wc * 32 + cofs);
 #pragma unroll
   for (int mi = 0; mi < 8; ++mi) {
     const long long m = row0 + wr * 128 + mi * 16 + (lane & 15);
     float v0[8], v1[8];
     row8(acc[mi][0], acc[mi][1], v0);
     row8(acc[mi][2], acc[mi][3], v1);
-    if constexpr (MODE == GATED) {
-      gated_store<TY>(p, m, col0 + wc * 32 + cofs, b, v0, v1);
-    } else {
-      plain_store<TY>(p, m, col0 + wc * 64 + cofs, 0, v0);
-      plain_store<TY>(p, m, col0 + wc * 64 + 32 + cofs, 0, v1);
-    }
+    plain_store<TY>(p, m, col0 + wc * 64 + cofs, 0, v0);
+    plain_store<TY>(p, m, col0 + wc * 64 + 32 + cofs, 0, v1);
   }
-}
-
-// tiles go to the XCDs (workgroup id mod 8) in contiguous runs, and within a run eight row tiles take turns over the
-// column tiles, so that the 32 tiles in flight on an XCD share 8 row panels and 4 column panels in its L2
-__device__ __forceinline__ int tile_of(int bid, int nwg) {
-  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, loc = bid >> 3;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + loc;
-}
-__device__ __forceinline__ void place(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int per = 8 * tiles_n, g = id / per, in = id - g * per;
-  const int h = tiles_m - g * 8 < 8 ? tiles_m - g * 8 : 8;
-  tn = in / h;
-  tm = g * 8 + (in - tn * h);
 }
 
 // ----------------------------------------------------------------------------------------------------- a few rows of x
@@ -611,33 +719,29 @@ __global__ __launch_bounds__(512, 2) void gated_big_kernel(GatedP p, Share sh, f
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x4 acc[8][4];
   int tm, tn;
-  if (MODE == GATED || (int)blockIdx.x < sh.whole) {
-    place(tile_of(blockIdx.x, MODE == GATED ? gridDim.x : sh.whole), sh.tiles_m, sh.tiles_n, tm, tn);
-    const long long row0 = (long long)tm * 256;
-    const int col0 = tn * (MODE == GATED ? 128 : 256);
-    tile256<TY, MODE>(p, row0, col0, 0, sh.steps, acc, lds, wave, lane);
-    store256<TY, MODE>(p, row0, col0, acc, wave, lane);
+  if ((int)blockIdx.x < sh.whole) {
+    place(tile_of(blockIdx.x, sh.whole), sh.tiles_m, sh.tiles_n, tm, tn);
+    tile256<TY, MODE>(p, (long long)tm * 256, tn * 256, 0, sh.steps, acc, lds, wave, lane);
+    store256<TY>(p, (long long)tm * 256, tn * 256, acc, wave, lane);
     return;
   }
-  if constexpr (MODE != GATED) {
-    const int w = tile_of(blockIdx.x - sh.whole, sh.wgs);
-    auto job = [&](int t, int kb, int n, int slot) {
-      place(sh.whole + t, sh.tiles_m, sh.tiles_n, tm, tn);
-      tile256<TY, MODE>(p, (long long)tm * 256, tn * 256, kb, n, acc, lds, wave, lane);
-      GatedP q = p;
-      q.C = part + (long long)slot * 65536;
-      q.ldc = 256;
-      q.c_type = T_F32;
-      q.M = q.N = 256;
-      store256<TY, MODE>(q, 0, 0, acc, wave, lane);
-    };
-    const int j = w / sh.rest, kb = part_start(sh, j);
-    job(w - j * sh.rest, kb, part_start(sh, j + 1) - kb, w);
-    if (w < sh.over * sh.runs) {
-      const int l = w / sh.runs, i = w - l * sh.runs, k0 = part_start(sh, sh.splits - 1), len = sh.steps - k0;
-      const int from = (int)((long long)i * len / sh.runs), to = (int)((long long)(i + 1) * len / sh.runs);
-      job(sh.rest - sh.over + l, k0 + from, to - from, sh.wgs + w);
-    }
+  const int w = tile_of(blockIdx.x - sh.whole, sh.wgs);
+  GatedP q = p;  // a partial tile
+  q.ldc = 256;
+  q.c_type = T_F32;
+  q.M = q.N = 256;
+  const int j = w / sh.rest;
+  int t = w - j * sh.rest, kb = part_start(sh, j), n = part_start(sh, j + 1) - kb;
+  for (int slot = w;; slot = sh.wgs + w) {
+    place(sh.whole + t, sh.tiles_m, sh.tiles_n, tm, tn);
+    tile256<TY, MODE>(p, (long long)tm * 256, tn * 256, kb, n, acc, lds, wave, lane);
+    q.C = part + (long long)slot * 65536;
+    store256<TY>(q, 0, 0, acc, wave, lane);
+    if (slot >= sh.wgs || w >= sh.over * sh.runs) break;
+    const int l = w / sh.runs, i = w - l * sh.runs, k0 = part_start(sh, sh.splits - 1), len = sh.steps - k0;
+    t = sh.rest - sh.over + l;
+    kb = k0 + (int)((long long)i * len / sh.runs);
+    n = k0 + (int)((long long)(i + 1) * len / sh.runs) - kb;
   }
 }
 
@@ -856,17 +960,16 @@ JoinJob join_job(TileJob& j, void* ws) {
 
 // Shares a product of 256 x 256 tiles out where that is shorter, in K-steps of a workgroup (1.75 us with the chip full): a
 // partial tile's way to memory and back takes 0.07 of them (256 KiB twice at 4 TB/s), second jobs and launches 4
-Share share_out(Mode mode, long long M, long long N, long long K) {
+Share share_out(long long M, long long N, long long K) {
   Share s = {};
-  const int per = mode == GATED ? 128 : 256;
   s.tiles_m = (int)((M + 255) / 256);
-  s.tiles_n = (int)((N + per - 1) / per);
+  s.tiles_n = (int)((N + 255) / 256);
   s.steps = (int)((K + 63) / 64);
   const long long tiles = (long long)s.tiles_m * s.tiles_n;
   s.rest = (int)(tiles % 256);
   s.whole = (int)tiles;
   s.splits = 1;
-  if (mode == GATED || s.rest == 0) return s;
+  if (s.rest == 0) return s;
   int splits = (255 + s.rest) / s.rest;
   if (splits > s.steps / 4) splits = s.steps / 4;
   if (splits < 2) return s;
@@ -909,15 +1012,20 @@ int forward(const GatedP& p, hipStream_t s) {
     hipLaunchKernelGGL((gated_few_kernel<TY>), dim3((unsigned)((p.N + 31) / 32)), dim3(64 * FEW_WAVES), 0, s, p);
     return 0;
   }
-  // The tile: 256 x 256 once its tiles fill more than half of the 256 CUs, 128 x 128 once its own fill most of them (two
-  // fit a CU), else 64 x 64. Measured (bf16, us; 256 / 128 / 64): 2048 x 1024 x 2736 31 / 40 / 51, 2048 x 768 x 2048
-  // (128 tiles) 23.0 / 21.0 / 29, 512 x 1280 x 3416 (54, 216) 30 / 22 / 29, 512 x 768 x 2048 (16, 128) 21 / 13.8 / 10.5
-  const Share sh = share_out(GATED, p.M, p.N, p.K);
-  if (sh.whole >= 150 && near(p.lda) && near(p.ldb)) return product_big<TY, GATED>(p, sh, nullptr, s);
+  // The tile: 128 rows x 128 features once its tiles fill most of the 256 CUs, 128 x 64 once those fill them, else 64 x 32.
+  // Measured (bf16, us): 2048 x 1024 x 2736 28 / 38 / 51, 1024 x 1280 x 3416 (216 large tiles) 29.1 / 30.6 / 48,
+  // 4096 x 256 x 688 (192) 10.6 / 9.8 / 11.2, 512 x 1280 x 3416 (108, 216) 27 / 22.5 / 29, 512 x 768 x 2048 (64, 128)
+  // - / 13.8 / 10.5
+  const int64_t duo_m = ((int64_t)p.M + 127) / 128, duo_n = ((int64_t)p.N + 127) / 128;
+  OCTSAM_CHECK_ARG(duo_m * duo_n < (1 << 26), "gated_fwd: too many tiles");
+  if (duo_m * duo_n >= 200 && near(p.lda) && near(p.ldb)) {
+    (void)hipFuncSetAttribute((const void*)gated_duo_kernel<TY>, hipFuncAttributeMaxDynamicSharedMemorySize, DUO_LDS);
+    hipLaunchKernelGGL((gated_duo_kernel<TY>), dim3((unsigned)(duo_m * duo_n)), dim3(256), DUO_LDS, s, p, (int)duo_m, (int)duo_n);
+    return 0;
+  }
   GatedP q = p;
   q.kper = (p.K + 63) / 64 * 64;
   const int64_t large = ((int64_t)p.M + 127) / 128 * (((int64_t)p.N + 63) / 64), small = ((int64_t)p.M + 63) / 64 * (((int64_t)p.N + 31) / 32);
-  OCTSAM_CHECK_ARG(small < (1ll << 31), "gated_fwd: too many tiles");
   if (large >= 192)
     hipLaunchKernelGGL((gated_tile_kernel<TY, 128>), dim3((unsigned)large), dim3(256), 0, s, q, (p.N + 63) / 64);
   else
@@ -927,9 +1035,9 @@ int forward(const GatedP& p, hipStream_t s) {
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 // bytes of fp32 partials of a product
-int64_t partial_bytes(Mode mode, int64_t M, int64_t N, int64_t K, const TilePlan& t) {
+int64_t partial_bytes(int64_t M, int64_t N, int64_t K, const TilePlan& t) {
   if (M <= 0 || N <= 0) return 0;
-  const Share sh = share_out(mode, M, N, K);
+  const Share sh = share_out(M, N, K);
   const int64_t big = t.T == 256 ? (int64_t)(sh.wgs + sh.over * sh.runs) * 65536 * 4 : 0;
   GatedP p = {};
   p.M = (int)M;
@@ -965,9 +1073,9 @@ BwdPlan bwd_plan(int64_t M, int64_t D, int64_t F, bool x_q8) {
   at += round16((int64_t)b.slabs * 2 * F * 4);
   b.join_x = at;
   b.tiles = tile_plan(M, D, F);
-  at += partial_bytes(NN, M, D, 2 * F, b.tiles);
+  at += partial_bytes(M, D, 2 * F, b.tiles);
   b.join_w = at;
-  at += partial_bytes(TN, 2 * F, D, M, b.tiles);
+  at += partial_bytes(2 * F, D, M, b.tiles);
   b.total = at;
   return b;
 }
@@ -990,7 +1098,7 @@ int run_bwd(const BwdPlan& b, const ActBwd& act, int gu_type, const void* x, int
   px.N = pw.N = D;
   px.B = w, px.ldb = ldw, px.C = dx, px.ldc = lddx, px.c_type = TY, px.M = (int)M, px.K = 2 * F;
   pw.B = x, pw.ldb = ldx, pw.C = dw, pw.ldc = lddw, pw.c_type = dw_type, pw.M = 2 * F, pw.K = (int)M;
-  const Share shx = share_out(NN, M, D, 2 * F), shw = share_out(TN, 2 * F, D, M);
+  const Share shx = share_out(M, D, 2 * F), shw = share_out(2 * F, D, M);
   const bool big = b.tiles.T == 256 && near(px.lda), big_x = big && near(ldw), big_w = big && M > 0 && near(ldx);
   if (dx && M > 0 && big_x)
     if (int rc = product_big<TY, NN>(px, shx, ws + b.join_x, s)) return rc;
