@@ -229,15 +229,15 @@ def call(name: str, *args) -> None:
         check(rc, name)
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """call() on device's current stream, whichever device is current (a launch goes to the current device)."""
-    index = device.index
+def call_on(index: int, name: str, *args) -> None:
+    """call() on the current stream of the device with this index, whichever device is current (a launch goes to the
+    current device)."""
     if index == torch._C._cuda_getDevice():
         rc = getattr(_lib or load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
         if rc:
             check(rc, name)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             call(name, *args)
 
 

@@ -234,8 +234,8 @@ def layernorm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: t
     return dx, dw, db
 
 
-# ---- 8-bit checkpoints, RMS norm, gated unit: tensors are [..., columns] with contiguous columns and, in two dimensions,
-# any row stride of at least their width; every launch goes to the operands' device, on its current stream
+# ---- 8-bit checkpoints, RMS norm, gated unit: tensors are [..., columns] with contiguous columns and, in two
+# dimensions, any row stride of at least their width; every launch goes to the operands' device, on its current stream
 
 _TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 _Q8 = 3  # the 8-bit form's type code
@@ -291,22 +291,23 @@ def _q8_pair(pair, rows, cols, what):
 
 
 def _device_of(first, *ts):
-    """The one device that all given tensors are on."""
-    dev = first.device
-    if dev.type != "cuda":
+    """The index of the one device that all given tensors are on."""
+    dev = first.get_device()
+    if dev < 0:
         raise ValueError("octsam kernels take device tensors only")
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"octsam kernels take device tensors only, all of one device: got {dev} and {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"octsam kernels take device tensors only, all of one device: got {first.device} and "
+                             f"{t.device}")
     return dev
 
 
 def q8_empty(shape, device) -> tuple[torch.Tensor, torch.Tensor]:
     """An unfilled 8-bit pair for [..., columns] values: float8_e4m3fn values of that shape and uint8 scales
     [..., ceil(columns / 32)] (scale byte b stands for 2^(b - 127) and multiplies 32 consecutive columns)."""
-    shape = tuple(shape)
-    return (torch.empty(shape, device=device, dtype=torch.float8_e4m3fn),
-            torch.empty(shape[:-1] + ((shape[-1] + 31) // 32,), device=device, dtype=torch.uint8))
+    *rows, cols = shape
+    return (torch.empty(*rows, cols, device=device, dtype=torch.float8_e4m3fn),
+            torch.empty(*rows, (cols + 31) // 32, device=device, dtype=torch.uint8))
 
 
 def quant8(x: torch.Tensor, q8=None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -317,7 +318,8 @@ def quant8(x: torch.Tensor, q8=None) -> tuple[torch.Tensor, torch.Tensor]:
     dev = _device_of(x, *q8)
     rows, cols, ldx = _rows(x, "x")
     q, ldq, scale, lds = _q8_pair(q8, rows, cols, "q8")
-    _lib.call_on(dev, "octsam_quant8", ptr(x), _type(x, "x"), ldx, rows, cols, ptr(q), ldq, ptr(scale), lds)
+    _lib.call_on(dev, "octsam_quant8", x.data_ptr(), _type(x, "x"), ldx, rows, cols, q.data_ptr(), ldq,
+                 scale.data_ptr(), lds)
     return q8
 
 
@@ -326,16 +328,17 @@ def dequant8(q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> torch.T
     dev = _device_of(q, scale, out)
     rows, cols, ldo = _rows(out, "out")
     q, ldq, scale, lds = _q8_pair((q, scale), rows, cols, "q")
-    _lib.call_on(dev, "octsam_dequant8", ptr(q), ldq, ptr(scale), lds, rows, cols, ptr(out), _type(out, "out"), ldo)
+    _lib.call_on(dev, "octsam_dequant8", q.data_ptr(), ldq, scale.data_ptr(), lds, rows, cols, out.data_ptr(),
+                 _type(out, "out"), ldo)
     return out
 
 
 def rmsnorm_fwd(x: torch.Tensor, w: torch.Tensor, eps: float, out: torch.Tensor | None = None, *,
                 residual: torch.Tensor | None = None, sum_out: torch.Tensor | None = None, q8=None,
                 rstd: torch.Tensor | None = None) -> torch.Tensor | None:
-    """out = RMS norm of s = x + residual over the last dim, times w (fp32); see octsam_rmsnorm_fwd. residual: x's type or
-    fp32; sum_out receives s in residual's type (it may be x or residual itself, in place); q8: an 8-bit pair that
-    receives out's values; rstd: fp32 [rows], for the backward. Every output is optional."""
+    """out = RMS norm of s = x + residual over the last dim, times w (fp32); see octsam_rmsnorm_fwd. residual: x's type
+    or fp32; sum_out receives s in residual's type (it may be x or residual itself, in place); q8: an 8-bit pair that
+    receives the norm's values; rstd: fp32 [rows], for the backward. Every output is optional."""
     q, scale = q8 if q8 is not None else (None, None)
     dev = _device_of(x, w, out, residual, sum_out, q, scale, rstd)
     rows, D, ldx = _rows(x, "x")
@@ -355,16 +358,16 @@ def rmsnorm_fwd(x: torch.Tensor, w: torch.Tensor, eps: float, out: torch.Tensor 
         q, ldq, scale, ldsc = _q8_pair(q8, rows, D, "q8")
     if rstd is not None:
         _vector(rstd, rows, "rstd")
-    _lib.call_on(dev, "octsam_rmsnorm_fwd", ptr(x), xt, ldx, ptr(residual), rt, ldr, ptr(w), rows, D, float(eps), ptr(sum_out),
-             lds, ptr(out), yt, ldy, ptr(q), ldq, ptr(scale), ldsc, ptr(rstd))
+    _lib.call_on(dev, "octsam_rmsnorm_fwd", x.data_ptr(), xt, ldx, ptr(residual), rt, ldr, w.data_ptr(), rows, D,
+                 float(eps), ptr(sum_out), lds, ptr(out), yt, ldy, ptr(q), ldq, ptr(scale), ldsc, ptr(rstd))
     return out
 
 
 def rmsnorm_bwd(dy: torch.Tensor, s, rstd: torch.Tensor, w: torch.Tensor, dx: torch.Tensor, *,
                 dres: torch.Tensor | None = None, dw: torch.Tensor | None = None):
-    """Gradients of rmsnorm_fwd: returns (dx, dw). s: the sum that was normalised (x without a residual), or an 8-bit pair
-    of it; rstd from the forward; dx (the gradient of x and of residual) = the norm's gradient + dres (dx's type: what
-    arrives at the sum from the residual stream); it may be dy or dres itself, in place. dw fp32, overwritten."""
+    """Gradients of rmsnorm_fwd: returns (dx, dw). s: the sum that was normalised (x without a residual), or an 8-bit
+    pair of it; rstd from the forward; dx (the gradient of x and of residual) = the norm's gradient + dres (dx's type:
+    what arrives at the sum from the residual stream); it may be dy or dres itself, in place. dw fp32, overwritten."""
     s8 = isinstance(s, (tuple, list))
     sv, sc = s if s8 else (s, None)
     dev = _device_of(dy, sv, sc, rstd, w, dx, dres, dw)
@@ -388,8 +391,9 @@ def rmsnorm_bwd(dy: torch.Tensor, s, rstd: torch.Tensor, w: torch.Tensor, dx: to
         _vector(dw, D, "dw")
     nbytes = _lib.load().octsam_rmsnorm_bwd_workspace(rows, D)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-    _lib.call_on(dev, "octsam_rmsnorm_bwd", ptr(dy), _type(dy, "dy"), lddy, ptr(sv), st, lds, ptr(sc), ldsc, ptr(rstd), ptr(w),
-             rows, D, ptr(dres), lddres, ptr(dx), xt, lddx, ptr(dw), ptr(ws), nbytes)
+    _lib.call_on(dev, "octsam_rmsnorm_bwd", dy.data_ptr(), _type(dy, "dy"), lddy, sv.data_ptr(), st, lds, ptr(sc),
+                 ldsc, rstd.data_ptr(), w.data_ptr(), rows, D, ptr(dres), lddres, dx.data_ptr(), xt, lddx,
+                 dw.data_ptr(), ptr(ws), nbytes)
     return dx, dw
 
 
@@ -415,9 +419,9 @@ def _kept(kept, ty, rows, F, what):
 
 def gated_fwd(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, act: int = _lib.ACT_SILU,
               bias: torch.Tensor | None = None, save=None) -> torch.Tensor:
-    """out = act(g) * u with [g | u] = x w^T + bias: x [M, D], w [2F, D] (gate rows first), out [M, F], all bf16 or all fp16;
-    bias fp32 [2F]; D and F multiples of 8. save keeps g and u for gated_bwd: [M, 2F] of x's type, or an 8-bit pair
-    q8_empty((M, 2, F)); see octsam_gated_fwd."""
+    """out = act(g) * u with [g | u] = x w^T + bias: x [M, D], w [2F, D] (gate rows first), out [M, F], all bf16 or all
+    fp16; bias fp32 [2F]; D and F multiples of 8. save keeps g and u for gated_bwd: [M, 2F] of x's type, or an 8-bit
+    pair q8_empty((M, 2, F)); see octsam_gated_fwd."""
     sv, sc = save if isinstance(save, (tuple, list)) else (save, None)
     dev = _device_of(x, w, out, bias, sv, sc)
     ty = _e16(x, "x")
@@ -434,8 +438,8 @@ def gated_fwd(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, act: int =
     st = ldsv = ldsc = 0
     if save is not None:
         sv, st, ldsv, sc, ldsc = _kept(save, ty, M, F, "save")
-    _lib.call_on(dev, "octsam_gated_fwd", ptr(x), ldx, ptr(w), ldw, ptr(bias), M, D, F, act, ty, ptr(out), ldh, ptr(sv), st, ldsv,
-             ptr(sc), ldsc)
+    _lib.call_on(dev, "octsam_gated_fwd", x.data_ptr(), ldx, w.data_ptr(), ldw, ptr(bias), M, D, F, act, ty,
+                 out.data_ptr(), ldh, ptr(sv), st, ldsv, ptr(sc), ldsc)
     return out
 
 
@@ -475,8 +479,9 @@ def gated_bwd(dh: torch.Tensor, saved, x, w: torch.Tensor, *, act: int = _lib.AC
         _vector(db, 2 * F, "db")
     nbytes = _lib.load().octsam_gated_bwd_workspace(M, D, F, int(xt == _Q8))
     ws = torch.empty(max(nbytes, 16), device=dev, dtype=torch.uint8)
-    _lib.call_on(dev, "octsam_gated_bwd", ptr(dh), lddh, ptr(sv), st, ldsv, ptr(sc), ldsc, ptr(xv), xt, ldx, ptr(xs), ldxs, ptr(w),
-             ldw, M, D, F, act, ty, ptr(h), ldh, ptr(dx), lddx, ptr(dw), wt, lddw, ptr(db), ptr(ws), nbytes)
+    _lib.call_on(dev, "octsam_gated_bwd", dh.data_ptr(), lddh, sv.data_ptr(), st, ldsv, ptr(sc), ldsc, ptr(xv), xt,
+                 ldx, ptr(xs), ldxs, w.data_ptr(), ldw, M, D, F, act, ty, ptr(h), ldh, ptr(dx), lddx, ptr(dw), wt,
+                 lddw, ptr(db), ptr(ws), nbytes)
 
 
 def vit_attention(qkv: torch.Tensor, out: torch.Tensor, rel_pos_h: torch.Tensor, rel_pos_w: torch.Tensor, *,
