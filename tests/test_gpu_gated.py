@@ -507,3 +507,99 @@ def test_two_graphs_share_nothing(k):
     for _, out, want, _, _ in sets:
         for name in want:
             assert torch.equal(out[name], want[name]), name
+
+
+# ------------------------------------------------------------------------------------------------------- far and apart
+def test_offsets_past_32_bits(k):
+    """Tensors of more than 2^31 elements: the first and the last rows are checked."""
+    rows, cols = 66000, 32768  # 2.16e9 elements
+    ends = [0, 1, 65535, 65536, rows - 1]
+    x = torch.zeros(rows, cols, device="cuda", dtype=BF)
+    x[ends] = rnd(1, len(ends), cols, dtype=BF)
+    q, s = k.quant8(x)
+    v, want = ref.q8(x[ends])
+    assert torch.equal(q[ends].double(), v) and torch.equal(s[ends], want)
+    back = k.dequant8(q, s, torch.empty_like(x))
+    assert torch.equal(back[ends].double(), ref.q8_value(v, want))
+    del q, s
+    w = 1 + 0.1 * rnd(2, cols)
+    rstd = torch.empty(rows, device="cuda")
+    k.rmsnorm_fwd(x, w, 1e-6, back, rstd=rstd)
+    _, wr, wy = ref.norm_fwd(x[ends], w, 1e-6)
+    c = (cols / 64 + 64) * U32
+    close(back[ends], wy, wy.abs() * (half_step(BF) + c) + tiny(BF))
+    dy = back
+    dy.zero_()
+    dy[ends] = rnd(3, len(ends), cols, dtype=BF)
+    _, dw = k.rmsnorm_bwd(dy, x, rstd, w, dy)
+    wx, ww, size, wsize = ref.norm_bwd(rnd(3, len(ends), cols, dtype=BF), x[ends], rstd[ends], w)
+    close(dy[ends], wx, wx.abs() * half_step(BF) + size * c + tiny(BF))
+    close(dw, ww, wsize * (rows + 64) * U32)
+
+
+def test_norm_offsets_past_32_bits_in_registers(k):
+    rows, d = 2 ** 21 + 3, 1032
+    ends = [0, 2 ** 20, rows - 2, rows - 1]
+    x = torch.zeros(rows, d, device="cuda", dtype=F16)
+    x[ends] = rnd(1, len(ends), d, dtype=F16)
+    w = 1 + 0.1 * rnd(2, d)
+    y, rstd = torch.empty_like(x), torch.empty(rows, device="cuda")
+    k.rmsnorm_fwd(x, w, 1e-6, y, rstd=rstd)
+    _, _, wy = ref.norm_fwd(x[ends], w, 1e-6)
+    close(y[ends], wy, wy.abs() * (half_step(F16) + 100 * U32) + tiny(F16))
+    dx, _ = k.rmsnorm_bwd(y, x, rstd, w, torch.empty_like(x))
+    wx, _, size, _ = ref.norm_bwd(y[ends], x[ends], rstd[ends], w)
+    close(dx[ends], wx, wx.abs() * half_step(F16) + size * 100 * U32 + tiny(F16))
+
+
+def test_gated_offsets_past_32_bits(k):
+    """M x 2F > 2^31: forward with both kinds of save, and the backward's rows and sums (zero rows but for the ends)."""
+    M, D, F = 400000, 32, 2752
+    ends = [0, 1, 131072, 200001, M - 1]
+    x = torch.zeros(M, D, device="cuda", dtype=BF)
+    xe, w, _ = exact_operands(7, len(ends), D, F, BF)
+    x[ends] = xe
+    gu, h = ref.gated_fwd(xe, w, "silu")
+    out = torch.empty(M, F, device="cuda", dtype=BF)
+    kept = torch.empty(M, 2 * F, device="cuda", dtype=BF)
+    k.gated_fwd(x, w, out, save=kept)
+    g, u = gu[:, :F], gu[:, F:]
+    close(out[ends], h, h.abs() * half_step(BF) + (g.abs() + 1) * u.abs() * 8 * U32 + tiny(BF))
+    assert torch.equal(kept[ends].float(), gu.to(BF).float())
+    eight = k.q8_empty((M, 2, F), "cuda")
+    k.gated_fwd(x, w, out, save=eight)
+    v, s = ref.q8(gu.view(-1, F))
+    assert torch.equal(eight[0][ends].view(-1, F).double(), v) and torch.equal(eight[1][ends].view(len(s), -1), s)
+    dh = out
+    dh.zero_()
+    dh[ends] = rnd(8, len(ends), F, dtype=BF)
+    got = {"dx": torch.empty_like(x), "dw": torch.empty(2 * F, D, device="cuda"), "db": torch.empty(2 * F, device="cuda")}
+    for saved, full in ((kept, kept[ends]), (eight, ref.q8_value(eight[0][ends], eight[1][ends]).view(-1, 2 * F))):
+        k.gated_bwd(dh, saved, x, w, **got)
+        want = ref.gated_bwd(dh[ends], full, xe, w, "silu")
+        ours = dict(got, dx=got["dx"][ends])
+        check_bwd(ours, want, dh[ends], full, xe, w, BF, len(ends), F)
+        assert int((got["dx"] != 0).any(1).sum()) <= len(ends)
+
+
+def test_gated_strides_too_far_for_the_large_tiles(k):
+    """Row strides of 4 MiB and more take the smaller tiles: x in the forward, w in the backward (dw keeps the large)."""
+    far = 2 ** 21 + 8
+    M, D, F = 2500, 72, 1288
+    x, w, _ = exact_operands(3, M, D, F, BF)
+    near, out = torch.empty(M, F, device="cuda", dtype=BF), torch.empty(M, F, device="cuda", dtype=BF)
+    k.gated_fwd(x, w, near)
+    xf = torch.empty(M * far, device="cuda", dtype=BF).as_strided((M, D), (far, 1))
+    xf.copy_(x)
+    k.gated_fwd(xf, w, out)
+    assert torch.equal(out, near)  # (exact sums: the tile does not matter)
+    del xf
+    M, D, F = 16400, 520, 1032
+    x, w = rnd(1, M, D, dtype=BF), rnd(2, 2 * F, D, scale=D ** -0.5, dtype=BF)
+    dh, gu = rnd(3, M, F, dtype=BF), rnd(4, M, 2 * F, dtype=BF)
+    wf = torch.empty(2 * F * far, device="cuda", dtype=BF).as_strided((2 * F, D), (far, 1))
+    wf.copy_(w)
+    got = {"dx": torch.empty_like(x), "dw": torch.empty_like(w)}
+    k.gated_bwd(dh, gu, x, wf, **got)
+    want = ref.gated_bwd(dh, gu, x, w, "silu")
+    check_bwd(got, want, dh, gu, x, w, BF, M, F)
