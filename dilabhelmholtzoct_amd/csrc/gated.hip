@@ -784,7 +784,7 @@ __global__ __launch_bounds__(256) void gated_fix_kernel(GatedP p, Share sh, cons
 }
 
 // What is left after the products, in one launch: the K splits' fp32 partials of dx and dw added in order and rounded
-// once (a thread: 8 columns), and the row slabs' partial sums of db (a workgroup: 32 columns).
+// once (a thread: 8 columns), and the row slabs' partial sums of db (a workgroup: SUM_COLS columns).
 struct JoinJob {
   const float* part;
   void* out;
@@ -818,7 +818,7 @@ template <int TY>
 __global__ __launch_bounds__(256) void gated_finish_kernel(JoinJob x, JoinJob w, DbJob d) {
   if (blockIdx.x < x.blocks) return join_block<TY>(x, blockIdx.x);
   if (blockIdx.x < x.blocks + w.blocks) return join_block<TY>(w, blockIdx.x - x.blocks);
-  column_sums(d.part, d.slabs, d.n, (blockIdx.x - x.blocks - w.blocks) * 32, d.out);
+  column_sums(d.part, d.slabs, d.n, (blockIdx.x - x.blocks - w.blocks) * SUM_COLS, d.out);
 }
 
 // --------------------------------------------------------------------------------------------- element-wise backward
@@ -1122,7 +1122,7 @@ int run_bwd(const BwdPlan& b, const ActBwd& act, int gu_type, const void* x, int
     d.out = db;
     d.slabs = b.slabs;  // (none without rows: db is zero)
     d.n = 2 * F;
-    d.blocks = (unsigned)((d.n + 31) / 32);
+    d.blocks = (unsigned)((d.n + SUM_COLS - 1) / SUM_COLS);
   }
   if (const unsigned blocks = fx.blocks + fw.blocks + d.blocks)
     hipLaunchKernelGGL((gated_finish_kernel<TY>), dim3(blocks), dim3(256), 0, s, fx, fw, d);

@@ -99,21 +99,22 @@ __device__ __forceinline__ void store1(void* base, long long i, float v) {
 inline bool type_ok(int t) { return t >= 0 && t <= 2; }
 inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 
-// Column sums of `rows` fp32 rows in fixed order by a workgroup of 256: 32 columns from c0 on, eight rows at a time (many
-// loads in flight: the sum is a chain of latencies otherwise).
+// Column sums of `rows` fp32 rows in fixed order by a workgroup of 256: SUM_COLS columns from c0 on, sixteen rows at a time
+// (many loads in flight: the sum is a chain of latencies otherwise).
+constexpr int SUM_COLS = 16;
 __device__ __forceinline__ void column_sums(const float* __restrict__ part, int rows, int cols, int c0, float* __restrict__ out) {
-  __shared__ float fold[8][32];
-  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5, c = c0 + lane;
+  __shared__ float fold[16][SUM_COLS];
+  const int lane = threadIdx.x & 15, sub = threadIdx.x >> 4, c = c0 + lane;
   float t = 0.0f;
   if (c < cols) {
 #pragma unroll 8
-    for (int k = sub; k < rows; k += 8) t += part[(long long)k * cols + c];
+    for (int k = sub; k < rows; k += 16) t += part[(long long)k * cols + c];
   }
   fold[sub][lane] = t;
   __syncthreads();
   if (sub == 0 && c < cols) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) t += fold[k][lane];
+    for (int k = 1; k < 16; ++k) t += fold[k][lane];
     out[c] = t;
   }
 }

@@ -104,6 +104,9 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(NormFwd a) {
   __shared__ float red[4];
   const int lane = threadIdx.x % T;
   const float inv_d = 1.0f / (float)a.D;
+  float w[NCH][8];
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) load_chunk<T_F32, T, W>(a.w, 0, lane, c, a.D, w[c]);
   const long long last = (a.rows + RPB - 1) / RPB * RPB;  // (all lanes of a wave run every pass: they reduce together)
   for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / T; row < last; row += (long long)gridDim.x * RPB) {
     const int D = row < a.rows ? a.D : 0;  // (a row past the end has no columns; it loads the last row's)
@@ -133,10 +136,8 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(NormFwd a) {
     if (D && lane == 0 && a.rstd) a.rstd[row] = rstd;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      float w[8];
-      load_chunk<T_F32, T, W>(a.w, 0, lane, c, a.D, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * rstd * w[e];
+      for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * rstd * w[c][e];
       cut_chunk<T, W>(lane, c, D, v[c]);
       if (a.y) store_chunk_by<T, W>(a.y_type, a.y, row * a.ldy, lane, c, D, v[c]);
       if (a.q) {  // (uniform)
@@ -377,10 +378,10 @@ __global__ __launch_bounds__(256) void rmsnorm_dw_any_kernel(NormBwd a) {
 
 // dw from the workgroups' partial rows (none: zero)
 __global__ __launch_bounds__(256) void dw_sum_kernel(const float* part, int rows, int D, float* dw) {
-  column_sums(part, rows, D, blockIdx.x * 32, dw);
+  column_sums(part, rows, D, blockIdx.x * SUM_COLS, dw);
 }
 
-constexpr int MAX_BLOCKS = 1024;  // workgroups of the backward, i.e. partial rows of dw
+constexpr int MAX_BLOCKS = 512;  // workgroups of the backward, i.e. partial rows of dw
 
 bool vec_ok(const void* p, long long ld, int bytes) { return !p || (ld % 8 == 0 && aligned(p, bytes)); }
 
@@ -487,7 +488,7 @@ extern "C" int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy,
   OCTSAM_CHECK_ARG(dw, "rmsnorm_bwd: null operand");
   const hipStream_t st = (hipStream_t)stream;
   if (rows == 0) {
-    hipLaunchKernelGGL(dw_sum_kernel, dim3((unsigned)((D + 31) / 32)), dim3(256), 0, st, (const float*)nullptr, 0, D, dw);
+    hipLaunchKernelGGL(dw_sum_kernel, dim3((unsigned)((D + SUM_COLS - 1) / SUM_COLS)), dim3(256), 0, st, (const float*)nullptr, 0, D, dw);
     OCTSAM_LAUNCH_CHECK("octsam_rmsnorm_bwd");
     return 0;
   }
@@ -514,7 +515,7 @@ extern "C" int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy,
   if (dy_type == T_BF16) { RUN(T_BF16) } else if (dy_type == T_F32) { RUN(T_F32) } else { RUN(T_F16) }
 #undef RUN
   if (nb > 1)
-    hipLaunchKernelGGL(dw_sum_kernel, dim3((unsigned)((D + 31) / 32)), dim3(256), 0, st, (const float*)workspace, nb, D, dw);
+    hipLaunchKernelGGL(dw_sum_kernel, dim3((unsigned)((D + SUM_COLS - 1) / SUM_COLS)), dim3(256), 0, st, (const float*)workspace, nb, D, dw);
   OCTSAM_LAUNCH_CHECK("octsam_rmsnorm_bwd");
   return 0;
 }
