@@ -1050,7 +1050,7 @@ int64_t partial_bytes(int64_t M, int64_t N, int64_t K, const TilePlan& t) {
 
 // rows per workgroup of the element-wise backward (grid y: at most 32768 workgroups)
 int64_t slab_of(int64_t M) {
-  const int64_t least = (M + 32767) / 32768, want = M <= 2048 ? 8 : M <= 8192 ? 32 : 64;
+  const int64_t least = (M + 32767) / 32768, want = M <= 2048 ? 8 : 32;
   return least > want ? (least + 7) / 8 * 8 : want;
 }
 
