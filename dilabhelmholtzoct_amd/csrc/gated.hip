@@ -15,6 +15,7 @@
 // [k][x] (W in dx, both in dW) use the same loops: the second kind is read from LDS with the transposing 64-bit read.
 #include "q8.h"
 #include <math.h>
+#include <type_traits>
 #include "../../include/octsam.h"
 
 namespace {
@@ -493,8 +494,10 @@ __global__ __launch_bounds__(256, 2) void gated_duo_kernel(GatedP p, int tiles_m
 // c ^ 2 ((r & 3) << 1 | (r >> 3) & 1): a transposing read's 32 lanes (rows q of 4, and 8 + q) cover 16 chunk slots, and
 // a fragment's address is one xor of a lane constant with the column block, plus constants.
 // 16384 x 5472 x 1024 (dx) 152 us, 1210 TFLOP/s, MFMAs busy 60 % at the 2.0 GHz that the chip holds. What bounds it is the
-// way of every K-step's new lines into the XCD's L2: the DMA alone, nothing computed, takes 147 us (out of L2 it could
-// run at half that), fragment reads alone 67. Three stages of B did not shorten it.
+// sum of the parts on one SIMD pair: DMA alone 147 us here (70 for the same addresses without the kernel's other work),
+// fragment reads alone 67, reads and MFMAs 118. Three stages of B did not shorten it, nor did 32x32x16 MFMAs; scalar work
+// kept out of the loop (descriptors by addition, a loop for each wave row) and the MFMA segments' priority took dw of
+// 16384 x 1280 x 3416 from 287 to 257 us.
 constexpr int STAGE = 65536;
 
 template <int TY, bool KM>
@@ -513,6 +516,24 @@ __device__ __forceinline__ typename Elem<TY>::v8 frag256(const char* img, int x0
   }
 }
 
+// A [k][x] operand's rows from K-step to K-step: the descriptor of the 64 rows at hand (fewer at K's end: the others read as
+// zero), from column x0 of xdim on. Kept by addition: the loop's scalar instructions stand in the way of its loads
+struct StepRows {
+  const char* at;
+  long long step;  // bytes of 64 rows
+  int ld2, width, left;
+  __device__ __forceinline__ StepRows(const void* X, long long ld, long long x0, long long xdim, int k, int K)
+      : at((const char*)X + (long long)k * ld * 2 + x0 * 2), step(ld * 128), ld2((int)ld * 2), width((int)(xdim - x0) * 2), left(K - k) {}
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows() const {
+    const int bytes = ((left < 64 ? left : 64) - 1) * ld2 + width;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, bytes > 0 ? bytes : 0, 0x00020000);
+  }
+  __device__ __forceinline__ void next() {
+    at += step;
+    left -= 64;
+  }
+};
+
 // acc = the tile at (row0, col0) over the K-steps [kb, kb + n), n >= 1
 template <int TY, int MODE>
 __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col0, int kb, int n, f32x4 (&acc)[8][4], char* lds,
@@ -520,63 +541,65 @@ __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col
   typedef typename Elem<TY>::v8 v8;
   constexpr bool AKM = MODE == TN;  // (B is [k][x] in both)
   const int wr = wave >> 2, wc = wave & 3;
-  const long long lda2 = p.lda * 2, ldb2 = p.ldb * 2;
-  const char *A = (const char*)p.A, *B = (const char*)p.B;
+  const int lda2 = (int)p.lda * 2, ldb2 = (int)p.ldb * 2;
   // a lane's part of a 1 KiB DMA piece j. k in rows: 8 rows of 128 B, by j & 1; [k][x]: 4 rows of 256 B, by (j >> 1) & 1
   // (the part of the chunk swizzle that the piece number gives)
-  int va[2], vb[2];
-  auto lane_part = [&](bool km, int e, long long ld2) {
-    if (km) return (int)((lane >> 4) * ld2) + (((lane & 15) ^ (((lane >> 4) << 2) | (e << 1))) << 4);
+  int va[2], vb[2], kc[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
     const int r = e * 8 + (lane >> 3);
-    return (int)(r * ld2) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
-  };
+    kc[e] = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+    const int cols = ((lane & 15) ^ (((lane >> 4) << 2) | (e << 1))) << 4;
+    va[e] = AKM ? (lane >> 4) * lda2 + cols : r * lda2 + kc[e] * 2;
+    vb[e] = (lane >> 4) * ldb2 + cols;
+  }
+  StepRows sa(p.A, p.lda, row0, p.M, kb * 64, p.K), sb(p.B, p.ldb, col0, p.N, kb * 64, p.K);
+  const __amdgpu_buffer_rsrc_t ra = range((const char*)p.A + row0 * p.lda * 2, (p.M - row0 < 256 ? p.M - row0 : 256) * p.lda * 2);
+  // pieces [j0, j0 + N) of half h of A (16 a half), stage t; s: A's rows of that stage
+  auto load_a = [&](const StepRows& s, int h, int j0, int t, auto count) __attribute__((always_inline)) {
+    char* dst = lds + (t & 1) * STAGE + h * 16384 + j0 * 1024;
+    const int k = (kb + t) * 64;
+    int v[2] = {va[0], va[1]};
+    if (!AKM && k + 64 > p.K) {  // (a K that is no multiple of 64: chunks past it)
 #pragma unroll
-  for (int e = 0; e < 2; ++e) va[e] = lane_part(AKM, e, lda2);
+      for (int e = 0; e < 2; ++e) v[e] = k + kc[e] < p.K ? va[e] : OUT_OF_RANGE;
+    }
+    const __amdgpu_buffer_rsrc_t rs = AKM ? s.rows() : ra;
+    const int at = AKM ? j0 * 4 * lda2 + h * 256 : (h * 128 + j0 * 8) * lda2 + k * 2;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) vb[e] = lane_part(true, e, ldb2);
-  const __amdgpu_buffer_rsrc_t ra = range(A + row0 * lda2, (p.M - row0 < 256 ? p.M - row0 : 256) * lda2);
-  // 16-B chunk of a row of k that lies past K (only in the last K-step of a K that is no multiple of 64)
-  auto cut = [&](int v, int e, int t) {
-    const int r = e * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-    return (kb + t) * 64 + 64 <= p.K || (kb + t) * 64 + c * 8 < p.K ? v : OUT_OF_RANGE;
+    for (int i = 0; i < decltype(count)::value; ++i)  // (j0 is even)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(dst + i * 1024), 16, v[AKM ? ((j0 + i) >> 1) & 1 : i & 1],
+                                               at + (AKM ? i * 4 : (i & ~1) * 8) * lda2, 0, 0);
   };
-  auto km_range = [&](const char* X, long long ld2, long long x0, long long xdim, int t) {
-    const long long k = (long long)(kb + t) * 64, rows = p.K - k < 64 ? p.K - k : 64;
-    return range(X + k * ld2 + x0 * 2, (rows - 1) * ld2 + (xdim - x0) * 2);
+  // pieces [j0, j0 + N) of B (32, 16 to a half of 128 columns; j0 a multiple of 4)
+  auto load_b = [&](const StepRows& s, int j0, int t, auto count) __attribute__((always_inline)) {
+    char* dst = lds + (t & 1) * STAGE + 32768 + j0 * 1024;
+    const __amdgpu_buffer_rsrc_t rs = s.rows();
+    const int at = (j0 & 15) * 4 * ldb2 + (j0 >> 4) * 256;
+#pragma unroll
+    for (int i = 0; i < decltype(count)::value; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(dst + i * 1024), 16, vb[(i >> 1) & 1], at + i * 4 * ldb2, 0, 0);
   };
-  auto dma_a = [&](int h, int j, int t) {  // piece j (of 16) of A's half h, stage t
-    const lds_ptr_t dst = (lds_ptr_t)(lds + (t & 1) * STAGE + h * 16384 + j * 1024);
-    if constexpr (AKM)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(km_range(A, lda2, row0 + h * 128, p.M, t), dst, 16, va[(j >> 1) & 1], (int)(4 * j * lda2), 0, 0);
-    else
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, dst, 16, cut(va[j & 1], j & 1, t),
-                                               (int)((h * 128 + (j & ~1) * 8) * lda2) + (kb + t) * 128, 0, 0);
-  };
-  auto dma_b = [&](int j, int t) {  // piece j (of 32) of B, stage t
-    const lds_ptr_t dst = (lds_ptr_t)(lds + (t & 1) * STAGE + 32768 + j * 1024);
-    const int h = j >> 4, jj = j & 15;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(km_range(B, ldb2, col0 + h * 128, p.N, t), dst, 16, vb[(jj >> 1) & 1], (int)(4 * jj * ldb2), 0, 0);
-  };
+  using std::integral_constant;
 #pragma unroll
   for (int mi = 0; mi < 8; ++mi)
 #pragma unroll
     for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = (f32x4)0.0f;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) dma_a(0, wave * 2 + i, 0);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) dma_a(1, wave * 2 + i, 0);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) dma_b(wave * 4 + i, 0);
+  load_a(sa, 0, wave * 2, 0, integral_constant<int, 2>());
+  load_a(sa, 1, wave * 2, 0, integral_constant<int, 2>());
+  load_b(sb, wave * 4, 0, integral_constant<int, 4>());
+  sa.next();
+  sb.next();
   if (n > 1) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) dma_a(0, wave * 2 + i, 1);
+    load_a(sa, 0, wave * 2, 1, integral_constant<int, 2>());
     wait_loads<2>();
   } else {
     wait_loads<0>();
   }
   hard_barrier();
-  if (wr == 1) hard_barrier();
-  for (int t = 0; t < n; ++t) {
+  // (a loop for each wave row: nothing of one stands in the other's way)
+  auto step = [&](int t, auto row) __attribute__((always_inline)) {
+    constexpr int WR = decltype(row)::value;
     const char* cur = lds + (t & 1) * STAGE;
     v8 af[8][2], bf[4][2];
 #pragma unroll
@@ -586,39 +609,34 @@ __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col
         bf[ni][kh] = frag256<TY, true>(cur + 32768 + (wc >> 1) * 16384, (wc & 1) * 64 + ni * 16, kh, lane);
 #pragma unroll
       for (int mi = 0; mi < 8; ++mi) {
-        if constexpr (AKM) af[mi][kh] = frag256<TY, true>(cur + wr * 16384, mi * 16, kh, lane);
-        else af[mi][kh] = frag256<TY, false>(cur, wr * 128 + mi * 16, kh, lane);
+        if constexpr (AKM) af[mi][kh] = frag256<TY, true>(cur + WR * 16384, mi * 16, kh, lane);
+        else af[mi][kh] = frag256<TY, false>(cur, WR * 128 + mi * 16, kh, lane);
       }
     }
-    if (wr == 0) {
-      if (t + 1 < n) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dma_b(wc * 8 + i, t + 1);
-      }
+    if constexpr (WR == 0) {
+      if (t + 1 < n) load_b(sb, wc * 8, t + 1, integral_constant<int, 8>());
+      sb.next();
     } else {
-      if (t + 1 < n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dma_a(1, wc * 4 + i, t + 1);
-      }
-      if (t + 2 < n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dma_a(0, wc * 4 + i, t + 2);
-      }
+      if (t + 1 < n) load_a(sa, 1, wc * 4, t + 1, integral_constant<int, 4>());
+      sa.next();
+      if (t + 2 < n) load_a(sa, 0, wc * 4, t + 2, integral_constant<int, 4>());
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the fragments are in registers: the stage may be refilled)
-    if (wr == 1) {
+    if constexpr (WR == 1) {
       if (t + 2 < n) wait_loads<8>();
       else if (t + 1 < n) wait_loads<4>();
       else wait_loads<0>();
     }
     hard_barrier();
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
       for (int mi = 0; mi < 8; ++mi)
 #pragma unroll
         for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = mma<TY>(bf[ni][kh], af[mi][kh], acc[mi][ni]);
-    if (wr == 0) {
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (WR == 0) {
       wait_loads<0>();
       hard_barrier();
     } else {
@@ -626,6 +644,12 @@ __device__ __forceinline__ void tile256(const GatedP& p, long long row0, int col
       else wait_loads<0>();
       if (t + 1 < n) hard_barrier();
     }
+  };
+  if (wr == 0) {
+    for (int t = 0; t < n; ++t) step(t, integral_constant<int, 0>());
+  } else {
+    hard_barrier();
+    for (int t = 0; t < n; ++t) step(t, integral_constant<int, 1>());
   }
 }
 
