@@ -668,60 +668,127 @@ __device__ __forceinline__ void store256(const GatedP& p, long long row0, int co
 }
 
 // ----------------------------------------------------------------------------------------------------- a few rows of x
-// Up to 16 rows (serving: one token) the time is W's way from memory, so W is read once, straight into fragments and
-// with many loads in flight: a workgroup has 32 features (their gate and up rows), its eight waves take the K-steps of
-// 32 in turn (neighbours share 128-byte lines), load four steps at once, and their sums meet in LDS. Rows of x past M
-// read as zero. One row, 1280 x 3416 bf16: 7.8 us on the GPU against 9.8 on the tiles above, of which an empty launch
-// is about 3; 4 x 4096 x 11008: 42 us, 4.2 TB/s. From 17 rows on the tiles are as fast.
-constexpr int FEW_ROWS = 16, FEW_WAVES = 8, FEW_STEPS = 4;
+// Up to 16 MB rows (serving: one token, a batch of them) the time is W's way from memory, so W is read once, straight
+// into fragments and with many loads in flight: a workgroup has NF features (their gate and up rows; NF = 8: both in one
+// block of 16), its eight waves take the K-steps of 32 in turn (neighbours share 128-byte lines), load 8 / MB steps at
+// once, and their sums meet in LDS. Rows of x past M read as zero. NF: 32 where an 8-bit group has to stay together; else
+// 8 while that makes at most one workgroup for each CU, and 16. Measured on the GPU (bf16, us, W in cache / a new W each
+// call; NF = 8, 16, 32; an empty launch is about 2.5): one row, 768 x 2048 3.2 / 4.1, 3.8 / 4.6, 5.4 / 6.2;
+// 1280 x 3416 5.2 / 6.3, 4.9 / 6.2, 7.5 / 9.2; 4 x 4096 x 11008 33 / 40, 32 / 41, 41 / 52 (4.3 TB/s of a new W).
+constexpr int FEW_WAVES = 8;
 
+// four consecutive features of a row, with no 8-bit save
 template <int TY>
+__device__ __forceinline__ void gated_store4(const GatedP& p, long long m, int f, f32x4 g, f32x4 u) {
+  typedef typename Elem<TY>::t t;
+  typedef t t4 __attribute__((ext_vector_type(4)));
+  if (m >= p.M || f >= p.N) return;
+  if (p.bias) {
+    g += *(const f32x4*)(p.bias + f);
+    u += *(const f32x4*)(p.bias + p.N + f);
+  }
+  if (p.save_type != T_NONE) {
+    t4 kg, ku;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      kg[e] = (t)g[e];
+      ku[e] = (t)u[e];
+    }
+    *(t4*)((t*)p.save + m * p.ldsave + f) = kg;
+    *(t4*)((t*)p.save + m * p.ldsave + p.N + f) = ku;
+  }
+  t4 h;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float unused;
+    h[e] = (t)(act_value<false>(p.act, g[e], unused) * u[e]);
+  }
+  *(t4*)((t*)p.C + m * p.ldc + f) = h;
+}
+
+template <int TY, int NF, int MB>
 __global__ __launch_bounds__(64 * FEW_WAVES) void gated_few_kernel(GatedP p) {
   typedef typename Elem<TY>::v8 v8;
-  __shared__ f32x4 sums[FEW_WAVES][4][64];
+  constexpr int HALF = NF / 16, NB = NF == 8 ? 1 : 2 * HALF, FEW_STEPS = 8 / MB;
+  __shared__ f32x4 sums[FEW_WAVES][NB][MB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int f0 = blockIdx.x * 32;
+  const int f0 = blockIdx.x * NF;
   const int steps = (p.K + 31) / 32;
-  const bool ox = r < p.M;
-  const char* px = (const char*)p.A + ((ox ? r : 0) * p.lda + g * 8) * 2;
-  const char* pw[4];
-  bool ow[4];
+  const char *px[MB], *pw[NB];
+  bool ox[MB], ow[NB];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // gate features f0 .. f0 + 15, + 16 .. + 31, then the up rows of the same
-    const int f = f0 + (i & 1) * 16 + r;
-    ow[i] = f < p.N;
-    pw[i] = (const char*)p.B + (((long long)(i >> 1) * p.N + (ow[i] ? f : 0)) * p.ldb + g * 8) * 2;
+  for (int i = 0; i < MB; ++i) {
+    ox[i] = i * 16 + r < p.M;
+    px[i] = (const char*)p.A + ((ox[i] ? i * 16 + r : 0) * p.lda + g * 8) * 2;
   }
-  f32x4 acc[4] = {(f32x4)0.0f, (f32x4)0.0f, (f32x4)0.0f, (f32x4)0.0f};
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {  // gate rows in blocks of 16, then the up rows of the same features
+    const int f = NF == 8 ? f0 + (r & 7) : f0 + (i & (HALF - 1)) * 16 + r, up = NF == 8 ? r >> 3 : i >= HALF;
+    ow[i] = f < p.N;
+    pw[i] = (const char*)p.B + (((long long)up * p.N + (ow[i] ? f : 0)) * p.ldb + g * 8) * 2;
+  }
+  f32x4 acc[NB][MB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[j][i] = (f32x4)0.0f;
   for (int s0 = wave; s0 < steps; s0 += FEW_WAVES * FEW_STEPS) {
-    u32x4 w[FEW_STEPS][4], x[FEW_STEPS];
+    u32x4 w[FEW_STEPS][NB], x[FEW_STEPS][MB];
 #pragma unroll
     for (int k = 0; k < FEW_STEPS; ++k) {
       const long long at = (s0 + k * FEW_WAVES) * 64ll;
       const bool in = (s0 + k * FEW_WAVES) * 32 + g * 8 < p.K;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[k][j] = in && ow[j] ? *(const u32x4*)(pw[j] + at) : (u32x4)0u;
-      x[k] = in && ox ? *(const u32x4*)(px + at) : (u32x4)0u;
+      for (int j = 0; j < NB; ++j) w[k][j] = in && ow[j] ? *(const u32x4*)(pw[j] + at) : (u32x4)0u;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) x[k][i] = in && ox[i] ? *(const u32x4*)(px[i] + at) : (u32x4)0u;
     }
 #pragma unroll
     for (int k = 0; k < FEW_STEPS; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        acc[j] = mma<TY>(__builtin_bit_cast(v8, w[k][j]), __builtin_bit_cast(v8, x[k]), acc[j]);
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+          acc[j][i] = mma<TY>(__builtin_bit_cast(v8, w[k][j]), __builtin_bit_cast(v8, x[k][i]), acc[j][i]);
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) sums[wave][j][lane] = acc[j];
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < MB; ++i) sums[wave][j][i][lane] = acc[j][i];
   __syncthreads();
-  if (wave > 0) return;
+  if (wave >= MB) return;
+  f32x4 v[NB];  // of the wave's 16 rows
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < NB; ++j) {
+    v[j] = sums[0][j][wave][lane];
 #pragma unroll
-    for (int k = 1; k < FEW_WAVES; ++k) acc[j] += sums[k][j][lane];
-  const int cofs = 16 * (g & 1) + 8 * (g >> 1);
-  float v0[8], v1[8];
-  row8(acc[0], acc[1], v0);
-  row8(acc[2], acc[3], v1);
-  gated_store<TY>(p, r, f0 + cofs, load_bias(p, f0 + cofs), v0, v1);
+    for (int k = 1; k < FEW_WAVES; ++k) v[j] += sums[k][j][wave][lane];
+  }
+  const int m = wave * 16 + r;
+  if constexpr (NF == 32) {
+    const int cofs = 16 * (g & 1) + 8 * (g >> 1);
+    float v0[8], v1[8];
+    row8(v[0], v[1], v0);
+    row8(v[2], v[3], v1);
+    gated_store<TY>(p, m, f0 + cofs, load_bias(p, f0 + cofs), v0, v1);
+  } else if constexpr (NF == 16) {
+    gated_store4<TY>(p, m, f0 + 4 * g, v[0], v[1]);
+  } else {
+    f32x4 u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __shfl_xor(v[0][i], 32);
+    if (g < 2) gated_store4<TY>(p, m, f0 + 4 * g, v[0], u);
+  }
+}
+template <int TY, int MB>
+void forward_few16(const GatedP& p, hipStream_t s) {
+  if (p.N <= 8 * 256) hipLaunchKernelGGL((gated_few_kernel<TY, 8, MB>), dim3((unsigned)((p.N + 7) / 8)), dim3(64 * FEW_WAVES), 0, s, p);
+  else hipLaunchKernelGGL((gated_few_kernel<TY, 16, MB>), dim3((unsigned)((p.N + 15) / 16)), dim3(64 * FEW_WAVES), 0, s, p);
+}
+template <int TY, int MB>
+void forward_few(const GatedP& p, hipStream_t s) {
+  if (p.save_type != T_Q8) return forward_few16<TY, MB>(p, s);
+  hipLaunchKernelGGL((gated_few_kernel<TY, 32, MB>), dim3((unsigned)((p.N + 31) / 32)), dim3(64 * FEW_WAVES), 0, s, p);
 }
 
 // How a product's tiles meet the chip's 256 workgroups: `whole` tiles (a multiple of 256) are one workgroup's each. Of
@@ -1032,8 +1099,14 @@ bool near(int64_t ld) { return ld < (1 << 21); }
 
 template <int TY>
 int forward(const GatedP& p, hipStream_t s) {
-  if (p.M <= FEW_ROWS) {
-    hipLaunchKernelGGL((gated_few_kernel<TY>), dim3((unsigned)((p.N + 31) / 32)), dim3(64 * FEW_WAVES), 0, s, p);
+  // Up to 16 rows, and up to 64 where the 16-feature workgroups are at most one for each CU (8-bit saves, 32 features a
+  // workgroup: 32). Measured against the tiles (bf16, us): 32 x 1280 x 3416 7.2 / 11.2, 64 x 1024 x 4096 8.4 / 9.9,
+  // 64 x 1280 x 3416 9.6 / 11.3, 64 x 256 x 688 3.7 / 4.0, but 64 x 1024 x 5504 13.6 / 9.9, 32 x 4096 x 11008 45 / 39
+  const bool few = p.N <= 16 * 256;
+  if (p.M <= 16 || (few && p.M <= (p.save_type == T_Q8 ? 32 : 64))) {
+    if (p.M <= 16) forward_few<TY, 1>(p, s);
+    else if (p.M <= 32) forward_few<TY, 2>(p, s);
+    else forward_few16<TY, 4>(p, s);
     return 0;
   }
   // The tile: 128 rows x 128 features once its tiles fill most of the 256 CUs, 128 x 64 once those fill them, else 64 x 32.

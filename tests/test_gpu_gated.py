@@ -270,7 +270,9 @@ GATED_SHAPES = [(1, 8, 8), (1, 256, 688), (2, 72, 40), (7, 264, 96), (16, 1280, 
                 (65, 136, 72), (130, 512, 200), (257, 200, 264), (1029, 256, 688), (300, 768, 1032), (768, 72, 1288),
                 (2100, 328, 520),
                 # 128 x 128 tiles in the forward; 256 x 256
-                (520, 136, 3000), (2500, 72, 2056)]
+                (520, 136, 3000), (2500, 72, 2056),
+                # few rows, 16 features a workgroup with half of them in the last one, several rounds of K-steps
+                (3, 328, 2056), (16, 2120, 4104), (20, 1096, 2600), (50, 584, 4088), (64, 40, 4104), (32, 2064, 48)]
 # the backward on 128 x 128 tiles; on 256 x 256: K cut over idle workgroups with second jobs (dw), a rest of 4 tiles behind
 # 256 whole ones (dx) and parts that come out even (dw)
 GATED_LARGE = [(1100, 520, 1032), (16400, 520, 1032), (16400, 1024, 1024)]
