@@ -795,10 +795,10 @@ void forward_few(const GatedP& p, hipStream_t s) {
 // the `rest` others K is cut into `splits` parts, all tiles at the same places; of the rest * splits parts, in the order
 // part-major, the first `wgs` are a workgroup's first job each, so that what runs together on an XCD walks the same K
 // over neighbouring tiles and shares its panels in L2 (cut end to end into equal runs instead, every workgroup walked a
-// K of its own: dw of 16384 x 1280 x 3416 353 us, against 230). What is left, `over` tiles' last parts, is cut into
-// `runs` each, the second jobs of the first over * runs workgroups: more runs end sooner but each leaves a partial tile
-// of 256 KiB. All jobs leave fp32 partial tiles (slot w, then wgs + w), and gated_fix_kernel adds a tile's in order.
-// wgs = 0: every tile is whole.
+// K of its own: dw of 16384 x 1280 x 3416 took half as long again, 353 us to 230 on the same loop). What is left, `over`
+// tiles' last parts, is cut into `runs` each, the second jobs of the first over * runs workgroups: more runs end sooner
+// but each leaves a partial tile of 256 KiB. All jobs leave fp32 partial tiles (slot w, then wgs + w), and
+// gated_fix_kernel adds a tile's in order. wgs = 0: every tile is whole.
 struct Share {
   int tiles_m, tiles_n, steps, whole, rest, splits, wgs, over, runs;
 };
@@ -1004,8 +1004,10 @@ __global__ __launch_bounds__(256) void gated_act_bwd_kernel(ActBwd a) {
 // else on T x T tiles in one launch, `per` K-steps a workgroup, so that both run out at the same time and the chip has
 // about 512 (T = 128) or 1024 workgroups, at least 4 steps each. Counted from the sizes alone, whichever outputs are
 // asked for: alone and together they have the same bits. Measured (bf16, the whole backward, us; 256 / 128 / 64):
-// 16384 x 1024 x 2736 469 / 630 / -, 8192 x 768 x 2048 (12288 steps) 220 / 237 / -, 4096 x 1024 x 2736 (11136)
-// 177 / 183 / -, 4096 x 768 x 2048 160 / 101 / 134, 1024 x 768 x 2048 71 / 40 / 47, 128 x 1024 x 2736 43 / 27 / 24.6
+// 16384 x 1024 x 2736 449 / 634 / 903, 4096 x 1280 x 3416 (17200 steps) 242 / 229 / 332, 8192 x 768 x 2048 (12288)
+// 216 / 238 / 252, 4096 x 1024 x 2736 (11136) 175 / 174 / 226, 6144 x 768 x 2048 (9216) 189 / 141 / 198,
+// 2048 x 1280 x 3416 (8600) 147 / 130 / 176, 4096 x 768 x 2048 157 / 100 / 131, 1024 x 768 x 2048 68 / 40 / 47,
+// 128 x 1024 x 2736 41 / 27 / 24.3
 struct TilePlan {
   int T, per;  // T = 256: per is for strides that the 256 x 256 kernel does not reach, on 128 x 128 tiles
 };
