@@ -315,19 +315,30 @@ __global__ __launch_bounds__(256) void gated_tile_kernel(GatedP p, int tiles_n) 
   tile<TY, GATED, T>(p, tiles_n, blockIdx.x, 0, smem);
 }
 
-// both products of the backward in one launch: dx's tiles (each K split of all tiles in turn), then dw's
+// work items go to the XCDs (workgroup id mod 8) in contiguous runs
+__device__ __forceinline__ int tile_of(int bid, int nwg) {
+  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, loc = bid >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + loc;
+}
+
+// Both products of the backward in one launch, the one with the longer K runs first: its tiles (each K split of all tiles
+// in turn), then the other's, which fill the gaps at the end (8192 x 768 x 2048 uncut: 154 us against 218). A run's
+// tiles share their rows' panel and most of a split's columns in an XCD's L2: 2 to 6 % against tiles in the
+// workgroups' order (2048 x 1024 x 2736 102 -> 96 us). (The forward's tiles, with few rows, are as fast without.)
 struct TileJob {
   GatedP p;
   int tiles, tiles_n, splits;
 };
 template <int TY, int T>
-__global__ __launch_bounds__(256) void gated_pair_kernel(TileJob x, TileJob w) {
+__global__ __launch_bounds__(256) void gated_pair_kernel(TileJob x, TileJob w, bool w_first) {
   __shared__ __attribute__((aligned(16))) TileLds<T> smem;
+  const int nx = x.tiles * x.splits, nw = w.tiles * w.splits, from = w_first ? nw : 0;  // where dx's workgroups start
   int b = blockIdx.x;
-  if (b < x.tiles * x.splits) {
+  if (b >= from && b < from + nx) {
+    b = tile_of(b - from, nx);
     tile<TY, NN, T>(x.p, x.tiles_n, b % x.tiles, b / x.tiles, smem);
   } else {
-    b -= x.tiles * x.splits;
+    b = tile_of(w_first ? b : b - nx, nw);
     tile<TY, TN, T>(w.p, w.tiles_n, b % w.tiles, b / w.tiles, smem);
   }
 }
@@ -348,12 +359,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void* base, long l
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)(bytes > 0 ? bytes : 0), 0x00020000);
 }
 
-// tiles go to the XCDs (workgroup id mod 8) in contiguous runs, and within a run eight row tiles take turns over the
-// column tiles, so that what is in flight on an XCD shares row and column panels in its L2
-__device__ __forceinline__ int tile_of(int bid, int nwg) {
-  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, loc = bid >> 3;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + loc;
-}
+// within a run eight row tiles take turns over the column tiles, so that what is in flight on an XCD shares row and column
+// panels in its L2
 __device__ __forceinline__ void place(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int per = 8 * tiles_n, g = id / per, in = id - g * per;
   const int h = tiles_m - g * 8 < 8 ? tiles_m - g * 8 : 8;
@@ -1000,35 +1007,120 @@ __global__ __launch_bounds__(256) void gated_act_bwd_kernel(ActBwd a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
-// The backward's two products. On 256 x 256 tiles, a launch each, from 12000 K-steps of both together (47 for each CU);
-// else on T x T tiles in one launch, `per` K-steps a workgroup, so that both run out at the same time and the chip has
-// about 512 (T = 128) or 1024 workgroups, at least 4 steps each. Counted from the sizes alone, whichever outputs are
-// asked for: alone and together they have the same bits. Measured (bf16, the whole backward, us; 256 / 128 / 64):
-// 16384 x 1024 x 2736 449 / 634 / 903, 4096 x 1280 x 3416 (17200 steps) 242 / 229 / 332, 8192 x 768 x 2048 (12288)
-// 216 / 238 / 252, 4096 x 1024 x 2736 (11136) 175 / 174 / 226, 6144 x 768 x 2048 (9216) 189 / 141 / 198,
-// 2048 x 1280 x 3416 (8600) 147 / 130 / 176, 4096 x 768 x 2048 157 / 100 / 131, 1024 x 768 x 2048 68 / 40 / 47,
-// 128 x 1024 x 2736 41 / 27 / 24.3
-struct TilePlan {
-  int T, per;  // T = 256: per is for strides that the 256 x 256 kernel does not reach, on 128 x 128 tiles
-};
-int64_t tiles_of(int64_t M, int64_t N, int T) { return ((M + T - 1) / T) * ((N + T - 1) / T); }
-TilePlan tile_plan(int64_t M, int64_t D, int64_t F) {
-  auto units = [&](int T) { return tiles_of(M, D, T) * ((2 * F + 63) / 64) + tiles_of(2 * F, D, T) * ((M + 63) / 64); };
-  TilePlan t;
-  t.T = units(256) >= 12000 ? 256 : units(128) >= 2500 ? 128 : 64;
-  const int64_t slots = t.T == 64 ? 1024 : 512, per = (units(t.T == 64 ? 64 : 128) + slots - 1) / slots;
-  t.per = (int)(per < 4 ? 4 : per);
-  return t;
+// Shares a product of 256 x 256 tiles out where that is shorter, in K-steps of a workgroup (1.75 us with the chip full): a
+// partial tile's way to memory and back takes 0.07 of them (256 KiB twice at 4 TB/s), second jobs and launches 4.
+// time: the product's, in K-steps
+Share share_out(long long M, long long N, long long K, double& time) {
+  Share s = {};
+  s.tiles_m = (int)((M + 255) / 256);
+  s.tiles_n = (int)((N + 255) / 256);
+  s.steps = (int)((K + 63) / 64);
+  const long long tiles = (long long)s.tiles_m * s.tiles_n;
+  s.rest = (int)(tiles % 256);
+  s.whole = (int)tiles;
+  s.splits = 1;
+  time = (double)((tiles + 255) / 256) * s.steps;
+  if (s.rest == 0) return s;
+  int splits = (255 + s.rest) / s.rest;
+  if (splits > s.steps / 4) splits = s.steps / 4;
+  if (splits < 2) return s;
+  int wgs = s.rest * splits, over = 0, runs = 0;
+  const double part = (double)s.steps / splits, partial = 0.07;
+  double shared = part + 4;
+  if (wgs > 256) {
+    over = wgs - 256;
+    wgs = 256;
+    runs = (int)sqrt(part / (partial * over));  // part / runs + partial * over * runs at its least
+    const int most = 256 / over < (int)part / 2 ? 256 / over : (int)part / 2;
+    runs = runs > most ? most : runs;
+    runs = runs < 1 ? 1 : runs;
+    shared += part / runs;
+  }
+  shared += partial * (wgs + over * runs);
+  if (shared > s.steps) return s;
+  time = (double)(tiles / 256) * s.steps + shared;
+  s.splits = splits;
+  s.whole = (int)(tiles - s.rest);
+  s.wgs = wgs;
+  s.over = over;
+  s.runs = runs;
+  return s;
 }
-TileJob tile_job(const GatedP& p, const TilePlan& t) {
+
+// How the backward's two products are cut: 256 x 256 tiles and a launch each, or T x T tiles with K in sx and sw parts and
+// one launch for both. Counted from the sizes alone, whichever outputs are asked for: alone and together they have the
+// same bits.
+struct TilePlan {
+  int64_t M, D, F;
+  int T, sx, sw;  // T = 256: sx, sw are for strides that the 256 x 256 kernel does not reach, on 128 x 128 tiles
+};
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t tiles_of(int64_t M, int64_t N, int T) { return ceil_div(M, T) * ceil_div(N, T); }
+
+// the K-step at which the last job ends when n jobs of a steps, then m of b <= a, go to `slots` places in that order
+int64_t last_end(int64_t n, int64_t a, int64_t m, int64_t b, int64_t slots) {
+  const int64_t late = n % slots, early = slots - late, t0 = n / slots * a, t1 = t0 + a;  // early places are free at t0, the others at t1
+  const int64_t up = ceil_div(a, b), down = a / b;
+  const int64_t i = early * up >= m ? ceil_div(m, early) : ceil_div(m + late * up, slots);  // b-jobs in a row on an early place, if one ends last
+  const int64_t k = m > early * down ? ceil_div(m - early * down, slots) : 0;           // on a late place
+  const int64_t end = t0 + i * b < t1 + k * b ? t0 + i * b : t1 + k * b;
+  return late && end < t1 ? t1 : end;
+}
+
+// The plan of least estimated time. The estimate, in us behind the element-wise part: on T x T tiles, a part for the
+// K-step at which the last workgroup ends (with 512 of T = 128 or 1024 of 64 at a time), one for the mean steps of a
+// place, for the MB of partials written and read, and for the splits that a sum is made of; on 256 x 256 tiles, the steps
+// of share_out. Fitted to the times of 38 sizes (17 x 256 x 688 to 16384 x 768 x 2048, up to 54 plans each; 6 to 8 %
+// off); the plans are 3 % behind the best measured ones on the geometric mean, at most 12 %. Equal K-steps for every
+// workgroup instead, the whole backward in us: 8192 x 768 x 2048 209 to 170 here, 4096 x 512 x 1376 73 / 58,
+// 4096 x 1024 x 2736 170 / 156, 1029 x 512 x 1376 37 / 29, 1029 x 256 x 688 21.7 / 20.2, 2048 x 768 x 2048 58 / 60.
+// At least 4 steps a split, and no more than two rounds of jobs.
+TilePlan tile_plan(int64_t M, int64_t D, int64_t F) {
+  static thread_local TilePlan last = {};  // (asked for the workspace first, then for the launch)
+  if (last.T && last.M == M && last.D == D && last.F == F) return last;
+  TilePlan best = {M, D, F, 0, 1, 1};
+  double least = 0;
+  constexpr int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  const int64_t kx = ceil_div(2 * F, 64), kw = ceil_div(M > 0 ? M : 1, 64);
+  for (int T = 128; T >= 64; T -= 64) {
+    const bool wide = T == 128;
+    const int64_t slots = wide ? 512 : 1024, nx = tiles_of(M, D, T), nw = tiles_of(2 * F, D, T);
+    for (int sx : SPLITS) {
+      if (sx > 1 && (sx * 4 > kx || nx * sx > 2 * slots)) break;
+      for (int sw : SPLITS) {
+        if (sw > 1 && (sw * 4 > kw || nw * sw > 2 * slots)) break;
+        const int64_t lx = ceil_div(kx, sx), lw = ceil_div(kw, sw), jx = nx * sx, jw = nw * sw;
+        const int64_t end = lx >= lw ? last_end(jx, lx, jw, lw, slots) : last_end(jw, lw, jx, lx, slots);
+        const double mean = (double)(jx * lx + jw * lw) / slots;
+        const double mb = ((sx > 1 ? (double)sx * M * D : 0.0) + (sw > 1 ? (double)sw * 2 * F * D : 0.0)) * 8e-6;
+        const int most = sx > sw ? sx : sw;
+        const double us = wide ? 6.5 + 0.54 * end + 0.72 * mean + 0.13 * mb + 0.12 * most : 5.0 + 0.3 * end + 0.73 * mean + 0.135 * mb + 0.18 * most;
+        if (best.T == 0 || us < least) {
+          least = us;
+          best.T = T;
+          best.sx = sx;
+          best.sw = sw;
+        }
+      }
+    }
+  }
+  if (best.T == 128) {
+    double x, w;
+    share_out(M, D, 2 * F, x);
+    share_out(2 * F, D, M, w);
+    if (1.58 * (x + w) < least) best.T = 256;
+  }
+  last = best;
+  return best;
+}
+TileJob tile_job(const GatedP& p, int T, int splits) {
   TileJob j = {};
   j.p = p;
-  const int T = t.T == 64 ? 64 : 128;
   j.tiles_n = (p.N + T - 1) / T;
   j.tiles = (int)tiles_of(p.M, p.N, T);
-  const int steps = (p.K + 63) / 64, s = (steps + t.per / 2) / t.per;
-  j.splits = s < 1 ? 1 : s > 64 ? 64 : s;
-  j.p.kper = (steps + j.splits - 1) / j.splits * 64;
+  const int steps = (p.K + 63) / 64, len = steps > 0 ? (steps + splits - 1) / splits : 1;
+  j.splits = steps > 0 ? (steps + len - 1) / len : 1;
+  j.p.kper = len * 64;
   return j;
 }
 // its partials go to ws: what is left to do for the output that p names
@@ -1049,43 +1141,6 @@ JoinJob join_job(TileJob& j, void* ws) {
   p.ldc = p.N;
   p.c_type = T_F32;
   return f;
-}
-
-// Shares a product of 256 x 256 tiles out where that is shorter, in K-steps of a workgroup (1.75 us with the chip full): a
-// partial tile's way to memory and back takes 0.07 of them (256 KiB twice at 4 TB/s), second jobs and launches 4
-Share share_out(long long M, long long N, long long K) {
-  Share s = {};
-  s.tiles_m = (int)((M + 255) / 256);
-  s.tiles_n = (int)((N + 255) / 256);
-  s.steps = (int)((K + 63) / 64);
-  const long long tiles = (long long)s.tiles_m * s.tiles_n;
-  s.rest = (int)(tiles % 256);
-  s.whole = (int)tiles;
-  s.splits = 1;
-  if (s.rest == 0) return s;
-  int splits = (255 + s.rest) / s.rest;
-  if (splits > s.steps / 4) splits = s.steps / 4;
-  if (splits < 2) return s;
-  int wgs = s.rest * splits, over = 0, runs = 0;
-  const double part = (double)s.steps / splits, partial = 0.07;
-  double shared = part + 4;
-  if (wgs > 256) {
-    over = wgs - 256;
-    wgs = 256;
-    runs = (int)sqrt(part / (partial * over));  // part / runs + partial * over * runs at its least
-    const int most = 256 / over < (int)part / 2 ? 256 / over : (int)part / 2;
-    runs = runs > most ? most : runs;
-    runs = runs < 1 ? 1 : runs;
-    shared += part / runs;
-  }
-  shared += partial * (wgs + over * runs);
-  if (shared > s.steps) return s;
-  s.splits = splits;
-  s.whole = (int)(tiles - s.rest);
-  s.wgs = wgs;
-  s.over = over;
-  s.runs = runs;
-  return s;
 }
 
 template <int TY, int MODE>
@@ -1134,15 +1189,16 @@ int forward(const GatedP& p, hipStream_t s) {
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 // bytes of fp32 partials of a product
-int64_t partial_bytes(int64_t M, int64_t N, int64_t K, const TilePlan& t) {
+int64_t partial_bytes(int64_t M, int64_t N, int64_t K, int T, int most) {
   if (M <= 0 || N <= 0) return 0;
-  const Share sh = share_out(M, N, K);
-  const int64_t big = t.T == 256 ? (int64_t)(sh.wgs + sh.over * sh.runs) * 65536 * 4 : 0;
+  double time;
+  const Share sh = share_out(M, N, K, time);
+  const int64_t big = T == 256 ? (int64_t)(sh.wgs + sh.over * sh.runs) * 65536 * 4 : 0;
   GatedP p = {};
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
-  const int splits = tile_job(p, t).splits;
+  const int splits = tile_job(p, T == 64 ? 64 : 128, most).splits;
   const int64_t small = splits > 1 ? splits * M * N * 4 : 0;
   return round16(big > small ? big : small);
 }
@@ -1172,9 +1228,9 @@ BwdPlan bwd_plan(int64_t M, int64_t D, int64_t F, bool x_q8) {
   at += round16((int64_t)b.slabs * 2 * F * 4);
   b.join_x = at;
   b.tiles = tile_plan(M, D, F);
-  at += partial_bytes(M, D, 2 * F, b.tiles);
+  at += partial_bytes(M, D, 2 * F, b.tiles.T, b.tiles.sx);
   b.join_w = at;
-  at += partial_bytes(2 * F, D, M, b.tiles);
+  at += partial_bytes(2 * F, D, M, b.tiles.T, b.tiles.sw);
   b.total = at;
   return b;
 }
@@ -1197,7 +1253,8 @@ int run_bwd(const BwdPlan& b, const ActBwd& act, int gu_type, const void* x, int
   px.N = pw.N = D;
   px.B = w, px.ldb = ldw, px.C = dx, px.ldc = lddx, px.c_type = TY, px.M = (int)M, px.K = 2 * F;
   pw.B = x, pw.ldb = ldx, pw.C = dw, pw.ldc = lddw, pw.c_type = dw_type, pw.M = 2 * F, pw.K = (int)M;
-  const Share shx = share_out(M, D, 2 * F), shw = share_out(2 * F, D, M);
+  double time;
+  const Share shx = share_out(M, D, 2 * F, time), shw = share_out(2 * F, D, M, time);
   const bool big = b.tiles.T == 256 && near(px.lda), big_x = big && near(ldw), big_w = big && M > 0 && near(ldx);
   if (dx && M > 0 && big_x)
     if (int rc = product_big<TY, NN>(px, shx, ws + b.join_x, s)) return rc;
@@ -1209,11 +1266,12 @@ int run_bwd(const BwdPlan& b, const ActBwd& act, int gu_type, const void* x, int
   if (tile_x || tile_w) {
     const int T = b.tiles.T == 64 ? 64 : 128;
     OCTSAM_CHECK_ARG(tiles_of(M, D, T) + tiles_of(2 * F, D, T) < (1 << 24), "gated_bwd: too many tiles");
-    if (tile_x) jx = tile_job(px, b.tiles), fx = join_job(jx, ws + b.join_x);
-    if (tile_w) jw = tile_job(pw, b.tiles), fw = join_job(jw, ws + b.join_w);
+    if (tile_x) jx = tile_job(px, T, b.tiles.sx), fx = join_job(jx, ws + b.join_x);
+    if (tile_w) jw = tile_job(pw, T, b.tiles.sw), fw = join_job(jw, ws + b.join_w);
     const int blocks = jx.tiles * jx.splits + jw.tiles * jw.splits;
-    if (T == 64) hipLaunchKernelGGL((gated_pair_kernel<TY, 64>), dim3((unsigned)blocks), dim3(256), 0, s, jx, jw);
-    else hipLaunchKernelGGL((gated_pair_kernel<TY, 128>), dim3((unsigned)blocks), dim3(256), 0, s, jx, jw);
+    const bool w_first = jw.p.kper > jx.p.kper;
+    if (T == 64) hipLaunchKernelGGL((gated_pair_kernel<TY, 64>), dim3((unsigned)blocks), dim3(256), 0, s, jx, jw, w_first);
+    else hipLaunchKernelGGL((gated_pair_kernel<TY, 128>), dim3((unsigned)blocks), dim3(256), 0, s, jx, jw, w_first);
   }
   DbJob d = {};
   if (db) {

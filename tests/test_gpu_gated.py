@@ -273,9 +273,9 @@ GATED_SHAPES = [(1, 8, 8), (1, 256, 688), (2, 72, 40), (7, 264, 96), (16, 1280, 
                 (520, 136, 3000), (2500, 72, 2056),
                 # few rows, 16 features a workgroup with half of them in the last one, several rounds of K-steps
                 (3, 328, 2056), (16, 2120, 4104), (20, 1096, 2600), (50, 584, 4088), (64, 40, 4104), (32, 2064, 48)]
-# the backward on 128 x 128 tiles; on 256 x 256: K cut over idle workgroups with second jobs (dw), a rest of 4 tiles behind
-# 256 whole ones (dx) and parts that come out even (dw)
-GATED_LARGE = [(1100, 520, 1032), (16400, 520, 1032), (16400, 1024, 1024)]
+# the backward on 128 x 128 tiles, dw's longer K runs first; on 256 x 256: K of both products' last tiles cut over idle
+# workgroups with second jobs, a rest of 4 tiles behind 256 whole ones (dx) and parts that come out even (dw)
+GATED_LARGE = [(1100, 520, 1032), (2300, 904, 1000), (16400, 520, 1032), (16400, 1032, 1544), (16400, 1024, 1024)]
 
 
 @pytest.mark.parametrize("M,D,F", GATED_SHAPES)
@@ -596,12 +596,14 @@ def test_gated_strides_too_far_for_the_large_tiles(k):
     k.gated_fwd(xf, w, out)
     assert torch.equal(out, near)  # (exact sums: the tile does not matter)
     del xf
-    M, D, F = 16400, 520, 1032
-    x, w = rnd(1, M, D, dtype=BF), rnd(2, 2 * F, D, scale=D ** -0.5, dtype=BF)
-    dh, gu = rnd(3, M, F, dtype=BF), rnd(4, M, 2 * F, dtype=BF)
-    wf = torch.empty(2 * F * far, device="cuda", dtype=BF).as_strided((2 * F, D), (far, 1))
-    wf.copy_(w)
-    got = {"dx": torch.empty_like(x), "dw": torch.empty_like(w)}
-    k.gated_bwd(dh, gu, x, wf, **got)
-    want = ref.gated_bwd(dh, gu, x, w, "silu")
-    check_bwd(got, want, dh, gu, x, w, BF, M, F)
+    for D, F in ((520, 1032), (1032, 1544)):
+        M = 16400
+        x, w = rnd(1, M, D, dtype=BF), rnd(2, 2 * F, D, scale=D ** -0.5, dtype=BF)
+        dh, gu = rnd(3, M, F, dtype=BF), rnd(4, M, 2 * F, dtype=BF)
+        wf = torch.empty(2 * F * far, device="cuda", dtype=BF).as_strided((2 * F, D), (far, 1))
+        wf.copy_(w)
+        got = {"dx": torch.empty_like(x), "dw": torch.empty_like(w)}
+        k.gated_bwd(dh, gu, x, wf, **got)
+        del wf
+        want = ref.gated_bwd(dh, gu, x, w, "silu")
+        check_bwd(got, want, dh, gu, x, w, BF, M, F)
