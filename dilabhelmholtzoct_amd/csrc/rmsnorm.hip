@@ -92,6 +92,14 @@ __device__ __forceinline__ float group_total(float v, float* red) {
   return v;
 }
 
+// v^(-1/2). 1 / sqrtf rounds twice, and a row's error goes into all of its values; a Newton step with the residue in two
+// parts takes it to about half a step (not where v is 0 or infinite)
+__device__ __forceinline__ float inverse_root(float v) {
+  const float r = 1.0f / sqrtf(v), h = v * r;
+  const float e = fmaf(-h, r, 1.0f) - fmaf(v, r, -h) * r;  // 1 - v r^2
+  return fabsf(e) < 1e-3f ? fmaf(0.5f * r, e, r) : r;
+}
+
 __device__ __forceinline__ void store1_by(int type, void* p, long long i, float v) {
   if (type == T_BF16) store1<T_BF16>(p, i, v);
   else if (type == T_F32) store1<T_F32>(p, i, v);
@@ -132,7 +140,7 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(NormFwd a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = fmaf(v[c][e], v[c][e], ss);
     ss = group_total<T>(ss, red);
-    const float rstd = 1.0f / sqrtf(fmaf(ss, inv_d, a.eps));
+    const float rstd = inverse_root(fmaf(ss, inv_d, a.eps));
     if (D && lane == 0 && a.rstd) a.rstd[row] = rstd;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -192,7 +200,7 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_any_kernel(NormFwd a) {
       ss = fmaf(v, v, ss);
     }
     ss = wave_sum(ss);
-    const float rstd = 1.0f / sqrtf(fmaf(ss, 1.0f / (float)a.D, a.eps));
+    const float rstd = inverse_root(fmaf(ss, 1.0f / (float)a.D, a.eps));
     if (lane == 0 && a.rstd) a.rstd[row] = rstd;
     for (int c0 = 0; c0 < a.D; c0 += 64) {
       const int c = c0 + lane;
