@@ -212,8 +212,8 @@ int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy, const void
  * Backward from the kept g, u (gu_type = type or 3): dg = dh * u * act'(g), du = dh * act(g); outputs, each optional:
  * h = act(g) * u again (for the weight gradient of the layer behind), dx = [dg | du] W (of `type`),
  * dw = [dg | du]^T x (fp32 or `type`; x of `type` or 8-bit, x_type 3), db = column sums of [dg | du] (fp32 [2F]).
- * Outputs are overwritten and must not overlap inputs. Fixed order of additions: the same bits every run. M = 0 gives
- * zero dw and db. workspace: octsam_gated_bwd_workspace(M, D, F, x_type == 3) bytes, 16-B aligned. */
+ * Outputs are overwritten and must not overlap inputs. Fixed order of additions, chosen by the sizes: the same bits every
+ * run. M = 0 gives zero dw and db. workspace: octsam_gated_bwd_workspace(M, D, F, x_type == 3) bytes, 16-B aligned. */
 int octsam_gated_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, int64_t M, int32_t D,
                      int32_t F, int32_t act, int32_t type, void* h, int64_t ldh, void* save, int32_t save_type,
                      int64_t ld_save, void* save_scale, int64_t ld_scale, void* stream);
