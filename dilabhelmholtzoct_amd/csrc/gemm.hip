@@ -2988,6 +2988,7 @@ extern "C" int OCTSAM_GEMM_ENTRY(const octsam_gemm_args* a, void* stream) {
                    a->M, a->N, a->K, a->batch);
   OCTSAM_CHECK_ARG(a->A && a->B && a->C, "octsam_gemm: null operand");
   OCTSAM_CHECK_ARG(a->a_mode >= 0 && a->a_mode <= 4 && a->b_mode >= 0 && a->b_mode <= 2, "octsam_gemm: bad mode");
+  OCTSAM_CHECK_ARG(a->act >= 0 && a->act <= OCTSAM_ACT_GELU, "octsam_gemm: activation %d (none, ReLU and GELU are here)", a->act);
   // K-contiguous operand loads move 8 consecutive k at a time; transposed loads move one k per chunk
   if (a->a_mode != 1 || a->b_mode == 0)
     OCTSAM_CHECK_ARG(a->K % 8 == 0, "octsam_gemm: K=%d must be a multiple of 8", a->K);

@@ -319,6 +319,7 @@ extern "C" int octsam_layernorm_fwd(const void* x, int32_t x_f32, const int32_t*
                                     int32_t act, float* mean, float* rstd, void* stream) {
   OCTSAM_CHECK_ARG(x && w && b && y && rows > 0, "octsam_layernorm_fwd: bad args");
   OCTSAM_CHECK_ARG((mean == nullptr) == (rstd == nullptr), "octsam_layernorm_fwd: mean/rstd both or neither");
+  OCTSAM_CHECK_ARG(act >= 0 && act <= OCTSAM_ACT_GELU, "octsam_layernorm_fwd: activation %d (none, ReLU and GELU are here)", act);
   OCTSAM_CHECK_ARG(aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b) && (!y2_f32 || aligned16(y2_f32)),
                    "octsam_layernorm_fwd: x, y, y2, w, b must be 16-B aligned");
   hipStream_t s = (hipStream_t)stream;
@@ -338,6 +339,7 @@ extern "C" int octsam_layernorm_bwd(const void* dy, int32_t dy_f32, const void* 
                                     float* db_part, int32_t nblocks, void* stream) {
   OCTSAM_CHECK_ARG(dy && x && mean && rstd && w && b && dx && dw_part && db_part && rows > 0 && nblocks > 0,
                    "octsam_layernorm_bwd: bad args");
+  OCTSAM_CHECK_ARG(act >= 0 && act <= OCTSAM_ACT_GELU, "octsam_layernorm_bwd: activation %d (none, ReLU and GELU are here)", act);
   OCTSAM_CHECK_ARG(aligned16(dy) && aligned16(x) && aligned16(dx) && aligned16(w) && aligned16(b) &&
                        (!dx2_bf16 || aligned16(dx2_bf16)),
                    "octsam_layernorm_bwd: dy, x, dx, dx2, w, b must be 16-B aligned");

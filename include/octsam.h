@@ -31,7 +31,7 @@ extern "C" {
 #define OCTSAM_ACT_NONE 0
 #define OCTSAM_ACT_RELU 1
 #define OCTSAM_ACT_GELU 2
-#define OCTSAM_ACT_SILU 3 /* x * sigmoid(x): the gated unit only */
+#define OCTSAM_ACT_SILU 3 /* x * sigmoid(x): the gated unit only; the GEMM and the layer norm refuse it */
 
 /* ---------------------------------------------------------------- library */
 int octsam_abi_version(void);
