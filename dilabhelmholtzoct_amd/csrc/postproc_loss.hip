@@ -150,6 +150,12 @@ __global__ __launch_bounds__(256) void dice_partials_kernel(const float* __restr
     part[((long long)m * gridDim.x + blockIdx.x) * 3 + tid] = red[tid][0] + red[tid][1] + red[tid][2] + red[tid][3];
 }
 
+// counts = 0 in front of confusion_kernel's atomics
+__global__ __launch_bounds__(256) void clear_counts_kernel(uint64_t* __restrict__ counts, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) counts[i] = 0;
+}
+
 // Per-map binary confusion counts of (x > 0) == (sigmoid(x) > 0.5) vs gt (evaluate_metrics,
 // ref:octsam/models/training_utils.py:126-156): counts[m] += (tp, fp, fn, tn), integer atomics (exact,
 // order-independent). One workgroup per (chunk, map), 16-B loads of 4 logits + 4 gt bytes per lane.
@@ -652,11 +658,8 @@ extern "C" int octsam_confusion(const float* masks, const uint8_t* gt, int32_t M
   OCTSAM_CHECK_ARG(masks && gt && counts && M >= 0 && HW > 0 && M <= 65535, "octsam_confusion: bad args");
   if (M == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
-  hipError_t e = hipMemsetAsync(counts, 0, (size_t)M * 4 * sizeof(uint64_t), s);
-  if (e != hipSuccess) {
-    octsam::set_error("octsam_confusion: memset failed: %s", hipGetErrorString(e));
-    return (int)e;
-  }
+  // (a kernel: a memory-set node of a captured graph has given wrong results on replays after the first)
+  hipLaunchKernelGGL(clear_counts_kernel, dim3((unsigned)((M * 4 + 255) / 256)), dim3(256), 0, s, counts, M * 4);
   const long long nb = (HW + 4095) / 4096;
   const int nblk = (int)(nb < 64 ? nb : 64);
   const long long chunk = (HW + nblk - 1) / nblk;
