@@ -216,10 +216,11 @@ def check(rc: int, what: str) -> None:
         raise OctsamError(f"{what} failed (code {rc}): {msg}")
 
 
-def stream_handle(device: torch.device | None = None) -> int:
-    """The current stream of device (default: the current device), without the cost of a Stream object."""
-    index = torch.cuda.current_device() if device is None or device.index is None else device.index
-    return torch._C._cuda_getCurrentRawStream(index)
+def stream_handle(device: torch.device | str | int | None = None) -> int:
+    """The current stream of device (default: the current device, without the cost of a Stream object)."""
+    if device is None:
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def call(name: str, *args) -> None:
