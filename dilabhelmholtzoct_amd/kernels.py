@@ -248,15 +248,23 @@ def _type(t, what):
     return ty
 
 
+def _width(n, what):
+    """n, a count that the entry takes in 32 bits (ctypes would cut it to them without a word)."""
+    if n > 0x7fffffff:
+        raise ValueError(f"{what}: a width of {n} does not fit the entries' 32 bits")
+    return n
+
+
 def _rows(t, what):
     """(rows, columns, row stride) of t seen as rows of its last dimension."""
     shape = t.shape
     if t.is_contiguous() and shape:
-        cols = shape[-1]
+        cols = _width(shape[-1], what)
         return (t.numel() // cols if cols else 0), cols, cols
     if len(shape) != 2:
         raise ValueError(f"{what}: [rows, columns] with any row stride, or contiguous [..., columns]")
     rows, cols = shape
+    _width(cols, what)
     ld, sc = t.stride()
     if sc != 1 and cols > 1:
         raise ValueError(f"{what}: columns must be contiguous")
@@ -429,7 +437,7 @@ def gated_fwd(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, act: int =
         raise ValueError("gated_fwd: x, w and out have one type")
     M, D, ldx = _rows(x, "x")
     n2, _, ldw = _rows(w, "w")
-    F = n2 // 2
+    F = _width(n2 // 2, "w")
     if w.dim() != 2 or n2 % 2 or w.shape[1] != D:
         raise ValueError(f"w is {tuple(w.shape)}: [2F, {D}] is expected")
     ldh = _like(out, M, F, "out")
