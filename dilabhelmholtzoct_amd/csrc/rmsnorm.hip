@@ -441,6 +441,11 @@ void launch_bwd(const NormBwd& a, bool vec, int nb, hipStream_t s) {
 #undef GO
 }
 
+// widest rows: the forward's columns count up in steps of 64 to below 2^31; a launch has fewer than 2^32 threads in a
+// dimension, 256 for 64 columns of rmsnorm_dw_any_kernel and for SUM_COLS of dw_sum_kernel (where there is more than one
+// partial row, or none)
+constexpr int MAX_FWD_D = 0x7fffffff - 63, MAX_BWD_D = (1 << 30) - 64, MAX_SUM_D = (1 << 28) - SUM_COLS;
+
 int bwd_blocks(int64_t rows) {
   const int64_t n = (rows + 15) / 16;
   return (int)(n < 1 ? 1 : n < MAX_BLOCKS ? n : MAX_BLOCKS);
@@ -454,6 +459,7 @@ extern "C" int octsam_rmsnorm_fwd(const void* x, int32_t x_type, int64_t ldx, co
                                   float* rstd, void* stream) {
   OCTSAM_CHECK_ARG(type_ok(x_type) && (!r || type_ok(r_type)) && (!y || type_ok(y_type)), "rmsnorm_fwd: unknown type");
   OCTSAM_CHECK_ARG(rows >= 0 && D > 0 && rows <= (1ll << 40), "rmsnorm_fwd: rows %lld, D %d", (long long)rows, D);
+  OCTSAM_CHECK_ARG(D <= MAX_FWD_D, "rmsnorm_fwd: D at most %d, got %d", MAX_FWD_D, D);
   if (rows == 0) return 0;
   OCTSAM_CHECK_ARG(x && w, "rmsnorm_fwd: null operand");
   OCTSAM_CHECK_ARG(!r || r_type == x_type || r_type == T_F32, "rmsnorm_fwd: the residual is fp32 or of x's type");
@@ -493,6 +499,8 @@ extern "C" int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy,
                                   float* dw, void* workspace, int64_t workspace_bytes, void* stream) {
   OCTSAM_CHECK_ARG(type_ok(dy_type) && type_ok(dx_type) && (type_ok(s_type) || s_type == T_Q8), "rmsnorm_bwd: unknown type");
   OCTSAM_CHECK_ARG(rows >= 0 && D > 0 && rows <= (1ll << 40), "rmsnorm_bwd: rows %lld, D %d", (long long)rows, D);
+  const int most = rows == 0 || bwd_blocks(rows) > 1 ? MAX_SUM_D : MAX_BWD_D;
+  OCTSAM_CHECK_ARG(D <= most, "rmsnorm_bwd: D at most %d for %lld rows, got %d", most, (long long)rows, D);
   OCTSAM_CHECK_ARG(dw, "rmsnorm_bwd: null operand");
   const hipStream_t st = (hipStream_t)stream;
   if (rows == 0) {

@@ -193,7 +193,8 @@ int octsam_dequant8(const void* q, int64_t ldq, const void* scale, int64_t ld_sc
  * Backward from the stored s (any type, or 8-bit with s_scale): dx = dres + rstd * (g - n * mean(g * n)), g = dy * w,
  * n = s * rstd, the gradient of x and of r; dres (optional, dx's type) is what arrives at s from the residual stream,
  * and dx may be dy or dres in place; dw[c] = sum over rows of dy * n (fp32, overwritten; fixed order of additions).
- * workspace: octsam_rmsnorm_bwd_workspace(rows, D) bytes (0: none is needed), 16-B aligned. */
+ * workspace: octsam_rmsnorm_bwd_workspace(rows, D) bytes (0: none is needed), 16-B aligned.
+ * D at most 2^31 - 64 forward, 2^28 - 16 backward (2^30 - 64 for 1 to 16 rows). */
 int octsam_rmsnorm_fwd(const void* x, int32_t x_type, int64_t ldx, const void* r, int32_t r_type, int64_t ldr,
                        const float* w, int64_t rows, int32_t D, float eps, void* sum_out, int64_t ld_sum, void* y,
                        int32_t y_type, int64_t ldy, void* q, int64_t ldq, void* scale, int64_t ld_scale, float* rstd,

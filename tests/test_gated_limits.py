@@ -39,3 +39,20 @@ def test_widths_past_32_bits(no_launch):
         with pytest.raises(ValueError, match="32 bits"):
             f()
             pytest.fail(f"case {i} was taken")
+
+
+P = 1 << 20  # a 16-B aligned address
+
+
+@pytest.mark.parametrize("rows,D", [(4, 2 ** 31 - 63), (4, 2 ** 31 - 1)])
+def test_norm_forward_width(rows, D):
+    lib = _lib.load()
+    assert lib.octsam_rmsnorm_fwd(P, 0, 1 << 32, None, 0, 0, P, rows, D, 1e-6, None, 0, P, 0, 1 << 32, None, 0, None, 0, None, None) != 0
+    assert b"D at most" in lib.octsam_last_error(), lib.octsam_last_error()
+
+
+@pytest.mark.parametrize("rows,D", [(0, 2 ** 28), (17, 2 ** 28 - 15), (1 << 20, 2 ** 31 - 1), (16, 2 ** 30 - 63), (1, 2 ** 31 - 1)])
+def test_norm_backward_width(rows, D):
+    lib = _lib.load()
+    assert lib.octsam_rmsnorm_bwd(P, 0, 1 << 32, P, 0, 1 << 32, None, 0, P, P, rows, D, None, 0, P, 0, 1 << 32, P, P, 1 << 62, None) != 0
+    assert b"D at most" in lib.octsam_last_error(), lib.octsam_last_error()
