@@ -7,10 +7,10 @@ F=$1
 cd "$(dirname "$0")/../dilabhelmholtzoct_amd/csrc"
 mkdir -p build/ab build/include
 git show HEAD:dilabhelmholtzoct_amd/csrc/$F > build/ab/old_$F
-cp common.h build/ab/ && cp ../../include/octsam.h build/include/
+cp common.h q8.h build/ab/ && cp ../../include/octsam.h build/include/
 sed -i 's#"../../include/octsam.h"#"../include/octsam.h"#' build/ab/old_$F
 EXTRA=""
 [ $F = vit_attention.hip ] && EXTRA="-mllvm -amdgpu-mfma-vgpr-form=1 -fno-honor-nans -mno-amdgpu-ieee"
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -Wall -Wno-unused-function $EXTRA -c build/ab/old_$F -o build/ab/old.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -fPIC -std=c++17 -Wall -Wno-unused-function $EXTRA -c build/ab/old_$F -o build/ab/old.o
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -o build/ab/liboctsam_old.so build/ab/old.o $(ls build/*.o | grep -v "build/${F}.o")
 ls -la build/ab/liboctsam_old.so

@@ -1,6 +1,6 @@
 // Micro-benchmark (diagnostics): an 8-wave 256x128-tile GEMM whose register epilogue of tile i runs inside the
 // main loop of tile i+1 (two accumulator sets per wave), against the library's octsam_gemm on the encoder shapes.
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 gemm8d.hip -o gemm8d -ldl ; run from the repo root.
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 gemm8d.hip -o gemm8d -ldl ; run from the repo root.
 #include <dlfcn.h>
 #include <hip/hip_runtime.h>
 

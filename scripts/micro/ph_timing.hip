@@ -1,4 +1,4 @@
-// Phase timing of the cubical-PH kernel (diagnostic): hipcc --offload-arch=gfx950 -O3 -DPH_PROFILE
+// Phase timing of the cubical-PH kernel (diagnostic): hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -DPH_PROFILE
 // -I. scripts/micro/ph_timing.hip -o scripts/micro/ph_timing_probe
 #include <cstdio>
 #include <cstdarg>

@@ -1,5 +1,5 @@
 // Cycles per edge of the union-find chunk resolve loop (cubical_ph.hip uf_wave) in instruction variants
-// (diagnostic): hipcc --offload-arch=gfx950 -O3 scripts/micro/uf_resolve_probe.hip -o scripts/micro/uf_resolve_probe
+// (diagnostic): hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 scripts/micro/uf_resolve_probe.hip -o scripts/micro/uf_resolve_probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #pragma clang diagnostic ignored "-Wunused-result"

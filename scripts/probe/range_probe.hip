@@ -1,6 +1,6 @@
 // Does the raw-buffer range check of an LDS-DMA buffer load include soffset? num_records = 4 rows of a [8][64] bf16
 // tile; lanes read rows 0..7 with the row offset in voffset (A) or in soffset (B: rows 4..7 via soffset = 4 rows).
-// Build: hipcc --offload-arch=gfx950 -O2 range_probe.hip -o range_probe. Diagnostic only.
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 range_probe.hip -o range_probe. Diagnostic only.
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

@@ -1,7 +1,7 @@
 // Probe of the LDS-DMA buffer load (16 B per lane) and ds_read_b64_tr_b16 as used by csrc/wgrad.hip: one wave
 // DMAs a [8 rows][64 columns] bf16 tile (value = 256 row + column) into LDS with the wgrad stage layout (64-B rows,
 // 512-B subtiles), dumps the LDS image, then every lane's transposed read at the wgrad fragment address.
-// Build: hipcc --offload-arch=gfx950 -O2 tr_probe.hip -o tr_probe. Diagnostic only.
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 tr_probe.hip -o tr_probe. Diagnostic only.
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>
