@@ -42,3 +42,13 @@ def test_comparison_builds_find_their_headers(source):
         script = f.read()
     for h in headers:
         assert h in script, h
+
+
+def test_build_compiles_where_a_library_is_there(monkeypatch):
+    """build() is the check that the sources compile: what is built already must not stand in for it."""
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: calls.append(cmd))
+    entry.build()
+    csrc = [c for c in calls if c[0] == "make" and any(str(a).endswith("csrc") for a in c)]
+    assert len(csrc) == 1 and "-B" in csrc[0]
