@@ -384,8 +384,10 @@ __device__ __forceinline__ void place(int id, int tiles_m, int tiles_n, int& tm,
 // fragments into registers; barrier; A's next stage and B's next but one on their way; 64 MFMAs. K is short here (D) and
 // the epilogue long (activation, product, 8-bit groups: about 25 vector operations per element of h): while one workgroup
 // is in its epilogue, its first loads, a wait or its fragment reads, the other has the matrix cores.
-// 16384 x 1024 x 2736 bf16: 161 us (1140 TFLOP/s), with the 8-bit save 181; the 256 x 256 tiles below, one workgroup to a
-// CU, took 174 and 193 (for the backward's longer K they are ahead: dx 152 us against 187, with two thirds of the reads).
+// 16384 x 1024 x 2736 bf16, medians with the chip kept busy: 186 us without a save (990 TFLOP/s), 206 with 16 bits, 221 with
+// 8 bits (the library's plain product of this shape, a pass of each in turn: 249). Timed in turn, the 256 x 256 tiles below,
+// one workgroup to a CU, took 8 % longer without a save and 7 % with 8 bits (for the backward's longer K they are ahead: dx
+// took a fifth less, with two thirds of the reads).
 // The fragment reads are assembly with their wait in the same block: as ordinary loads they would wait for all DMA in
 // flight.
 constexpr int DUO_B = 16384, DUO_LDS = 81920;
@@ -500,21 +502,23 @@ __global__ __launch_bounds__(256, 2) void gated_duo_kernel(GatedP p, int tiles_m
 
 // ----------------------------------------------------------------------------------------------------- 256 x 256 tile
 // The backward's large products: 256 x 256 x 64 tiles, eight waves as 2 (rows) x 4 (columns) with 128 x 64 each, operands
-// by LDS-DMA through buffer descriptors (what lies past an operand's end reads as zero), two stages of 64 KiB. A K-step of a wave is two segments between barriers: L reads its 24 fragments
-// and issues its share of the DMA, C runs its 64 MFMAs; the two wave rows run one segment apart, so that each SIMD has
-// one wave in its MFMAs while its other wave loads. A's rows 0-127 are read by wave row 0 alone (segment 2t), 128-255
-// by wave row 1 (2t + 1), B by both, and a region is refilled once its last reader has passed a barrier:
+// by LDS-DMA through buffer descriptors (what lies past an operand's end reads as zero), two stages of 64 KiB. A K-step of a
+// wave is two segments between barriers: L reads its 24 fragments and issues its share of the DMA, C runs its 64 MFMAs; the
+// two wave rows run one segment apart, so that each SIMD has one wave in its MFMAs while its other wave loads. A's rows
+// 0-127 are read by wave row 0 alone (segment 2t), 128-255 by wave row 1 (2t + 1), B by both, and a region is refilled once
+// its last reader has passed a barrier:
 //   wave row 0 in L(t): B(t + 1), landed at the end of its C(t)
 //   wave row 1 in L(t): A-hi(t + 1), landed at the end of its C(t); A-lo(t + 2), landed at the end of its L(t + 1)
 //   before the loop:    stage 0 and A-lo(1)
 // LDS images: rows of k as above; [k][x] operands as two halves of 128 columns, [64][256 B], chunk c of row r at
 // c ^ 2 ((r & 3) << 1 | (r >> 3) & 1): a transposing read's 32 lanes (rows q of 4, and 8 + q) cover 16 chunk slots, and
 // a fragment's address is one xor of a lane constant with the column block, plus constants.
-// 16384 x 5472 x 1024 (dx) 152 us, 1210 TFLOP/s, MFMAs busy 60 % at the 2.0 GHz that the chip holds. What bounds it is the
-// sum of the parts on one SIMD pair: DMA alone 147 us here (70 for the same addresses without the kernel's other work),
-// fragment reads alone 67, reads and MFMAs 118. Three stages of B did not shorten it, nor did 32x32x16 MFMAs; scalar work
-// kept out of the loop (descriptors by addition, a loop for each wave row) and the MFMA segments' priority took dw of
-// 16384 x 1280 x 3416 from 287 to 257 us.
+// 16384 x 5472 x 1024 (dx of 16384 x 1024 x 2736): median 160 us, 1150 TFLOP/s, MFMAs busy 55 % of the cycles at the 2.06 GHz
+// that the chip holds (the library's product, a pass of each in turn: 161); dw of the same sizes 185 (263). What bounds it is
+// the sum of the parts on one SIMD pair: of the loop's time then (152 us), copies of the kernel with the other parts left out
+// took 97 % with the DMA alone, 44 % with the fragment reads alone, 78 % with reads and MFMAs. Three stages of B did not
+// shorten it, nor did 32x32x16 MFMAs; scalar work kept out of the loop (descriptors by addition, a loop for each wave row)
+// and the MFMA segments' priority took a tenth off dw of 16384 x 1280 x 3416, which now takes 249 us (the library 429).
 constexpr int STAGE = 65536;
 
 template <int TY, bool KM>
@@ -812,7 +816,7 @@ void forward_few(const GatedP& p, hipStream_t s) {
 // the `rest` others K is cut into `splits` parts, all tiles at the same places; of the rest * splits parts, in the order
 // part-major, the first `wgs` are a workgroup's first job each, so that what runs together on an XCD walks the same K
 // over neighbouring tiles and shares its panels in L2 (cut end to end into equal runs instead, every workgroup walked a
-// K of its own: dw of 16384 x 1280 x 3416 took half as long again, 353 us to 230 on the same loop). What is left, `over`
+// K of its own: dw of 16384 x 1280 x 3416 took half as long again on the same loop). What is left, `over`
 // tiles' last parts, is cut into `runs` each, the second jobs of the first over * runs workgroups: more runs end sooner
 // but each leaves a partial tile of 256 KiB. All jobs leave fp32 partial tiles (slot w, then wgs + w), and
 // gated_fix_kernel adds a tile's in order. wgs = 0: every tile is whole.

@@ -3,6 +3,8 @@
 //
 // Layout: a lane owns 8 consecutive columns, so 4 lanes share a group (two xor-shuffles give its amax); widths that
 // are no multiple of 8 and strides or addresses off 16 bytes go element by element, 32 lanes a group.
+// Median times (us, bf16): 16384 x 2736 25.5 to 8 bits (136 MB) and 21.6 back (part of them from the last-level cache);
+// 16384 x 2731, element by element, 110 and 68: bound by the loads' and stores' count and the index's division, not by memory.
 #include "q8.h"
 #include "../../include/octsam.h"
 

@@ -16,6 +16,11 @@
 // multiple of 8 and strides and addresses off 16 bytes take the same kernels with single elements (W = 1: lane j holds
 // the columns j + T i, 32 lanes an 8-bit group). Rows over 8192 columns go column by column with a wave per row and are
 // read twice.
+//
+// Median times (us, bf16, residual, the chip kept busy): forward of 16384 x 1024 21.8 (134 MB, part of them still in the
+// last-level cache), with the 8-bit form 25.5; of 16384 x 1021 (single elements) 27.0, with the 8-bit form 46.3: there
+// the maxima over 32 lanes and single bytes are the time. Backward of 16384 x 1280 34.3 (168 MB) and 4.7 for dw; of
+// 16384 x 1021 26.7 from 16 bits (1024: 24.4), but 74 from 8 bits (1024: 22.8), a byte and its scale's byte a load.
 #include "q8.h"
 #include "../../include/octsam.h"
 

@@ -194,6 +194,7 @@ int octsam_dequant8(const void* q, int64_t ldq, const void* scale, int64_t ld_sc
  * n = s * rstd, the gradient of x and of r; dres (optional, dx's type) is what arrives at s from the residual stream,
  * and dx may be dy or dres in place; dw[c] = sum over rows of dy * n (fp32, overwritten; fixed order of additions).
  * workspace: octsam_rmsnorm_bwd_workspace(rows, D) bytes (0: none is needed), 16-B aligned.
+ * The squares are summed in fp32: a sum past fp32's largest number gives rstd = 0 and y = 0.
  * D at most 2^31 - 64 forward, 2^28 - 16 backward (2^30 - 64 for 1 to 16 rows). */
 int octsam_rmsnorm_fwd(const void* x, int32_t x_type, int64_t ldx, const void* r, int32_t r_type, int64_t ldr,
                        const float* w, int64_t rows, int32_t D, float eps, void* sum_out, int64_t ld_sum, void* y,
@@ -214,7 +215,8 @@ int octsam_rmsnorm_bwd(const void* dy, int32_t dy_type, int64_t lddy, const void
  * h = act(g) * u again (for the weight gradient of the layer behind), dx = [dg | du] W (of `type`),
  * dw = [dg | du]^T x (fp32 or `type`; x of `type` or 8-bit, x_type 3), db = column sums of [dg | du] (fp32 [2F]).
  * Outputs are overwritten and must not overlap inputs. Fixed order of additions, chosen by the sizes: the same bits every
- * run. M = 0 gives zero dw and db. workspace: octsam_gated_bwd_workspace(M, D, F, x_type == 3) bytes, 16-B aligned. */
+ * run. M = 0 gives zero dw and db. workspace: octsam_gated_bwd_workspace(M, D, F, x_type == 3) bytes, 16-B aligned (that of
+ * all outputs, whichever are asked for). M at most 2^30, D and F at most 2^24. */
 int octsam_gated_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, int64_t M, int32_t D,
                      int32_t F, int32_t act, int32_t type, void* h, int64_t ldh, void* save, int32_t save_type,
                      int64_t ld_save, void* save_scale, int64_t ld_scale, void* stream);
